@@ -8,8 +8,10 @@ include/kf_attn.h); this package is the Python host side.
   attention  torch-tensor API + the reference-compatible launcher
   multi_gpu  one-process-per-GPU sharding (batch / KV heads) and the
              cross-GPU split-KV decode (partials + NCCL all-gather + merge)
-  pointwise  RMSNorm (plain / fused residual), RoPE, SwiGLU
-             (C ABI: include/kf_pointwise.h)
+  pointwise  RMSNorm (plain / fused residual), RoPE, query/key norm with RoPE,
+             SwiGLU (C ABI: include/kf_pointwise.h)
+  kv_cache   paged KV cache held in 4 bits: write, read back, decode attention
+             over it (C ABI: include/kf_cache.h)
   synth      seeded counter-based N(0,1) fp16 inputs generated on the GPU
              (C ABI: include/kf_synth.h)
   build      nvcc build of the library (sm_100a only)
@@ -27,7 +29,8 @@ from .attention import (  # noqa: F401
     workspace_bytes,
 )
 
-from .pointwise import fused_add_rms_norm, rms_norm, rope_, swiglu  # noqa: F401
+from .kv_cache import flash_attn_paged_q4, kv_read_q4, kv_write_q4, q4_cache  # noqa: F401
+from .pointwise import fused_add_rms_norm, qk_norm_rope, rms_norm, rope_, swiglu  # noqa: F401
 from .synth import NormalStream, fill_normal_f16  # noqa: F401
 
 __version__ = "0.1.0"

@@ -1,5 +1,5 @@
 """ctypes binding of libkf_attn.so (the C ABI declared in include/kf_attn.h,
-include/kf_pointwise.h and include/kf_synth.h).
+include/kf_cache.h, include/kf_pointwise.h and include/kf_synth.h).
 
 There is no fallback: if the library is missing this module raises, and every
 compute entry point goes through the CUDA kernels in the library.
@@ -27,6 +27,9 @@ KF_FLAG_OUT_BF16 = 4
 KF_PW_BF16 = 1
 KF_ROPE_GPTJ = 2
 
+KF_CACHE_BF16 = 1
+KF_FLAG_Q_BF16 = 8
+
 # Every symbol include/kf_attn.h, include/kf_pointwise.h and include/kf_synth.h declare.
 EXPORTED = [
     "kf_strerror", "kf_last_cuda_error", "kf_version",
@@ -34,11 +37,14 @@ EXPORTED = [
     "kf_attn_workspace_bytes", "kf_attn_workspace_init", "kf_attn_plan",
     "kf_launch_flash_attn", "kf_attn_fwd_noalloc", "kf_device_error", "kf_set_wait_timeout_ns",
     "kf_selftest_wait_timeout",
-    "kf_rmsnorm", "kf_rope", "kf_swiglu",
+    "kf_rmsnorm", "kf_rope", "kf_qk_norm_rope", "kf_swiglu",
     "kf_peer_window_bytes", "kf_peer_window_alloc", "kf_peer_window_open", "kf_peer_window_close",
     "kf_peer_window_free", "kf_attn_exchange_combine", "kf_attn_fwd_exchange", "kf_attn_exchange_workspace_bytes",
     "kf_fill_normal_f16",
 ]
+
+# Every symbol include/kf_cache.h declares.
+EXPORTED_CACHE = ["kf_kv_write_q4", "kf_kv_read_q4", "kf_attn_fwd_paged_q4", "kf_attn_paged_q4_workspace_bytes"]
 
 KF_PEER_HANDLE_BYTES = 64
 KF_MAX_PEERS = 8
@@ -126,6 +132,16 @@ def lib():
     L.kf_rmsnorm.restype = I
     L.kf_rope.argtypes = [P, P, P, P, I, I, I, I, I, I, F, LL, LL, LL, LL, LL, LL, U, P]
     L.kf_rope.restype = I
+    L.kf_qk_norm_rope.argtypes = [P] * 8 + [I] * 6 + [F] * 3 + [LL] * 12 + [U, P]
+    L.kf_qk_norm_rope.restype = I
+    L.kf_kv_write_q4.argtypes = [P] * 4 + [I] * 6 + [LL] * 6 + [U, P]
+    L.kf_kv_write_q4.restype = I
+    L.kf_kv_read_q4.argtypes = [P] * 4 + [I] * 6 + [LL] * 6 + [U, P]
+    L.kf_kv_read_q4.restype = I
+    L.kf_attn_fwd_paged_q4.argtypes = [P] * 7 + [I] * 8 + [F, U, P, Z, P]
+    L.kf_attn_fwd_paged_q4.restype = I
+    L.kf_attn_paged_q4_workspace_bytes.argtypes = [I] * 7
+    L.kf_attn_paged_q4_workspace_bytes.restype = Z
     L.kf_swiglu.argtypes = [P, P, LL, I, U, P]
     L.kf_swiglu.restype = I
     L.kf_fill_normal_f16.argtypes = [P, LL, ctypes.c_ulonglong, LL, P]
@@ -136,5 +152,22 @@ def lib():
 
 
 def check(rc: int, what: str = "") -> None:
+    if rc != KF_OK:
+        raise KFError(rc, what)
+
+
+def on_device(index: int, fn, what: str, *args) -> None:
+    """``fn(*args, current stream of device index)`` with that device current; raises KFError on a status.
+
+    The two torch calls are the ones behind torch.cuda.current_stream / current_device, without
+    the Stream object and the lazy-initialisation check (a tensor on the device exists): the
+    small operators' host cost is mostly this."""
+    import torch
+
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != KF_OK:
         raise KFError(rc, what)

@@ -16,8 +16,11 @@
 #include <mutex>
 
 #include "../../include/kf_attn.h"
+#include "../../include/kf_cache.h"
 #include "../../include/kf_pointwise.h"
 #include "../../include/kf_synth.h"
+#include "cache_sm100.cuh"
+#include "decode_q4_sm100.cuh"
 #include "decode_sm100.cuh"
 #include "peer_sm100.cuh"
 #include "kf_ptx.cuh"
@@ -1323,6 +1326,22 @@ int swiglu_t(const kf::SwigluParams& p, cudaStream_t s) {
 }
 
 bool stride_ok(long long st) { return st >= 0 && st % 8 == 0; }
+bool strides_ok(long long b, long long h, long long s) { return stride_ok(b) && stride_ok(h) && stride_ok(s); }
+// The stride of a dimension of one element is never used; 0 keeps any value of it acceptable.
+void drop_unused_strides(int B, int H, int S, long long& b, long long& h, long long& s) {
+    if (B <= 1) b = 0;
+    if (H <= 1) h = 0;
+    if (S <= 1) s = 0;
+}
+
+template <bool BF16, bool NEOX>
+int qk_norm_rope_t(const kf::QkNormRopeParams& p, cudaStream_t s) {
+    int grid = 0;
+    int rc = pw_grid<kf::qk_norm_rope_kernel<BF16, NEOX>>(256, (p.n_tokens * (p.H_q + p.H_kv) + 7) / 8, &grid);
+    if (rc != KF_OK) return rc;
+    kf::qk_norm_rope_kernel<BF16, NEOX><<<grid, 256, 0, s>>>(p);
+    return launch_status();
+}
 
 }  // namespace
 
@@ -1410,6 +1429,62 @@ int kf_rope(void* q, void* k, const int* positions, const float* inv_freq, int B
     return bf16 ? rope_t<true, false>(p, hb, s) : rope_t<false, false>(p, hb, s);
 }
 
+int kf_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, void* q_out,
+                    void* k_out, const int* positions, const float* inv_freq, int B, int S, int H_q, int H_kv, int D,
+                    int rot_dim, float theta, float rot_scale, float eps, long long q_stride_b, long long q_stride_h,
+                    long long q_stride_s, long long k_stride_b, long long k_stride_h, long long k_stride_s,
+                    long long qo_stride_b, long long qo_stride_h, long long qo_stride_s, long long ko_stride_b,
+                    long long ko_stride_h, long long ko_stride_s, unsigned flags, void* stream) {
+    if (flags & ~static_cast<unsigned>(KF_PW_BF16 | KF_ROPE_GPTJ)) return KF_ERR_INVALID_ARG;
+    const bool neox = !(flags & KF_ROPE_GPTJ);
+    if (B < 0 || S < 0 || H_q < 0 || H_kv < 0 || H_q > 65535 || H_kv > 65535 || H_q + H_kv < 1) return KF_ERR_INVALID_ARG;
+    if (D < 16 || D > 512 || D % 16 != 0) return KF_ERR_INVALID_ARG;
+    if (rot_dim < 0 || rot_dim > D || rot_dim % (neox ? 16 : 8) != 0) return KF_ERR_INVALID_ARG;
+    if (rot_dim > 0 && !inv_freq && !(theta > 0.f && std::isfinite(theta))) return KF_ERR_INVALID_ARG;
+    if (!(eps >= 0.f) || !std::isfinite(eps) || !std::isfinite(rot_scale)) return KF_ERR_INVALID_ARG;
+    const long long n_tokens = static_cast<long long>(B) * S;
+    if (n_tokens == 0) return KF_OK;
+    drop_unused_strides(B, H_q, S, q_stride_b, q_stride_h, q_stride_s);
+    drop_unused_strides(B, H_q, S, qo_stride_b, qo_stride_h, qo_stride_s);
+    drop_unused_strides(B, H_kv, S, k_stride_b, k_stride_h, k_stride_s);
+    drop_unused_strides(B, H_kv, S, ko_stride_b, ko_stride_h, ko_stride_s);
+    if (H_q > 0 && (!q || !q_out || !strides_ok(q_stride_b, q_stride_h, q_stride_s) ||
+                    !strides_ok(qo_stride_b, qo_stride_h, qo_stride_s)))
+        return KF_ERR_INVALID_ARG;
+    if (H_kv > 0 && (!k || !k_out || !strides_ok(k_stride_b, k_stride_h, k_stride_s) ||
+                     !strides_ok(ko_stride_b, ko_stride_h, ko_stride_s)))
+        return KF_ERR_INVALID_ARG;
+    if ((H_q > 0 && (!aligned16(q) || !aligned16(q_out) || !aligned16(q_weight))) ||
+        (H_kv > 0 && (!aligned16(k) || !aligned16(k_out) || !aligned16(k_weight))))
+        return KF_ERR_MISALIGNED;
+    kf::QkNormRopeParams p;
+    p.q = static_cast<const uint16_t*>(q);
+    p.k = static_cast<const uint16_t*>(k);
+    p.qo = static_cast<uint16_t*>(q_out);
+    p.ko = static_cast<uint16_t*>(k_out);
+    p.qw = static_cast<const uint16_t*>(q_weight);
+    p.kw = static_cast<const uint16_t*>(k_weight);
+    p.pos = positions;
+    p.inv_freq = inv_freq;
+    p.q_sb = q_stride_b; p.q_sh = q_stride_h; p.q_ss = q_stride_s;
+    p.k_sb = k_stride_b; p.k_sh = k_stride_h; p.k_ss = k_stride_s;
+    p.qo_sb = qo_stride_b; p.qo_sh = qo_stride_h; p.qo_ss = qo_stride_s;
+    p.ko_sb = ko_stride_b; p.ko_sh = ko_stride_h; p.ko_ss = ko_stride_s;
+    p.n_tokens = n_tokens;
+    p.S = S;
+    p.H_q = H_q;
+    p.H_kv = H_kv;
+    p.D = D;
+    p.rot_dim = rot_dim;
+    p.eps = eps;
+    p.rot_scale = rot_scale;
+    p.log2_theta = inv_freq || rot_dim == 0 ? 0.0 : std::log2(static_cast<double>(theta));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool bf16 = flags & KF_PW_BF16;
+    if (neox) return bf16 ? qk_norm_rope_t<true, true>(p, s) : qk_norm_rope_t<false, true>(p, s);
+    return bf16 ? qk_norm_rope_t<true, false>(p, s) : qk_norm_rope_t<false, false>(p, s);
+}
+
 int kf_swiglu(const void* gate_up, void* out, long long rows, int inter, unsigned flags, void* stream) {
     if (flags & ~static_cast<unsigned>(KF_PW_BF16)) return KF_ERR_INVALID_ARG;
     if (rows < 0 || inter < 8 || inter % 8 != 0) return KF_ERR_INVALID_ARG;
@@ -1423,6 +1498,146 @@ int kf_swiglu(const void* gate_up, void* out, long long rows, int inter, unsigne
     p.ivec = inter / 8;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return (flags & KF_PW_BF16) ? swiglu_t<true>(p, s) : swiglu_t<false>(p, s);
+}
+
+}  // extern "C"
+
+// ---- 4-bit paged KV cache -----------------------------------------------------
+namespace {
+
+bool q4_dim_ok(int D) { return D == 64 || D == 128 || D == 256; }
+int log2_exact(int v) {
+    int l = 0;
+    while ((1 << l) < v) ++l;
+    return l;
+}
+
+int q4_io_params(const void* cache, const int* slots, const void* k, const void* v, int B, int S, int H_kv, int D,
+                 int n_blocks, int block_size, long long ksb, long long ksh, long long kss, long long vsb,
+                 long long vsh, long long vss, unsigned flags, kf::Q4IoParams* p) {
+    if (flags & ~static_cast<unsigned>(KF_CACHE_BF16)) return KF_ERR_INVALID_ARG;
+    if (B < 0 || S < 0 || H_kv <= 0 || H_kv > 65535 || n_blocks <= 0) return KF_ERR_INVALID_ARG;
+    if (!q4_dim_ok(D)) return KF_ERR_UNSUPPORTED_HEAD_DIM;
+    if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1))) return KF_ERR_INVALID_ARG;
+    drop_unused_strides(B, H_kv, S, ksb, ksh, kss);
+    drop_unused_strides(B, H_kv, S, vsb, vsh, vss);
+    if (!strides_ok(ksb, ksh, kss) || !strides_ok(vsb, vsh, vss)) return KF_ERR_INVALID_ARG;
+    if (static_cast<long long>(B) * S == 0) return KF_OK;
+    if (static_cast<long long>(B) * S > (1ll << 40)) return KF_ERR_INVALID_ARG;
+    if (!cache || !slots || !k || !v) return KF_ERR_INVALID_ARG;
+    if (!aligned16(cache) || !aligned16(k) || !aligned16(v)) return KF_ERR_MISALIGNED;
+    p->cache = static_cast<uint8_t*>(const_cast<void*>(cache));
+    p->slots = slots;
+    p->k = static_cast<uint16_t*>(const_cast<void*>(k));
+    p->v = static_cast<uint16_t*>(const_cast<void*>(v));
+    p->k_sb = ksb; p->k_sh = ksh; p->k_ss = kss;
+    p->v_sb = vsb; p->v_sh = vsh; p->v_ss = vss;
+    p->B = B;
+    p->S = S;
+    p->H = H_kv;
+    p->bs_log2 = log2_exact(block_size);
+    p->n_slots = static_cast<long long>(n_blocks) * block_size;
+    return KF_OK;
+}
+
+template <int D, bool BF16>
+int q4_io_launch(const kf::Q4IoParams& p, bool write, cudaStream_t s) {
+    const long long blocks = (2ll * p.B * p.S * p.H + 7) / 8;
+    int grid = 0;
+    int rc = write ? pw_grid<kf::q4_write_kernel<D, BF16>>(256, blocks, &grid)
+                   : pw_grid<kf::q4_read_kernel<D, BF16>>(256, blocks, &grid);
+    if (rc != KF_OK) return rc;
+    if (write) kf::q4_write_kernel<D, BF16><<<grid, 256, 0, s>>>(p);
+    else kf::q4_read_kernel<D, BF16><<<grid, 256, 0, s>>>(p);
+    return launch_status();
+}
+
+int q4_io(const kf::Q4IoParams& p, int D, bool bf16, bool write, void* stream) {
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (D) {
+        case 64: return bf16 ? q4_io_launch<64, true>(p, write, s) : q4_io_launch<64, false>(p, write, s);
+        case 128: return bf16 ? q4_io_launch<128, true>(p, write, s) : q4_io_launch<128, false>(p, write, s);
+        default: return bf16 ? q4_io_launch<256, true>(p, write, s) : q4_io_launch<256, false>(p, write, s);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int kf_kv_write_q4(const void* k, const void* v, void* cache, const int* slots, int B, int S, int H_kv, int D,
+                   int n_blocks, int block_size, long long k_stride_b, long long k_stride_h, long long k_stride_s,
+                   long long v_stride_b, long long v_stride_h, long long v_stride_s, unsigned flags, void* stream) {
+    kf::Q4IoParams p;
+    const int rc = q4_io_params(cache, slots, k, v, B, S, H_kv, D, n_blocks, block_size,
+                                k_stride_b, k_stride_h, k_stride_s, v_stride_b, v_stride_h, v_stride_s, flags, &p);
+    if (rc != KF_OK || static_cast<long long>(B) * S == 0) return rc;
+    return q4_io(p, D, flags & KF_CACHE_BF16, true, stream);
+}
+
+int kf_kv_read_q4(const void* cache, const int* slots, void* k, void* v, int B, int S, int H_kv, int D, int n_blocks,
+                  int block_size, long long k_stride_b, long long k_stride_h, long long k_stride_s,
+                  long long v_stride_b, long long v_stride_h, long long v_stride_s, unsigned flags, void* stream) {
+    kf::Q4IoParams p;
+    const int rc = q4_io_params(cache, slots, k, v, B, S, H_kv, D, n_blocks, block_size,
+                                k_stride_b, k_stride_h, k_stride_s, v_stride_b, v_stride_h, v_stride_s, flags, &p);
+    if (rc != KF_OK || static_cast<long long>(B) * S == 0) return rc;
+    return q4_io(p, D, flags & KF_CACHE_BF16, false, stream);
+}
+
+size_t kf_attn_paged_q4_workspace_bytes(int B, int H_q, int H_kv, int S_q, int D, int block_size, int max_blocks) {
+    (void)B; (void)H_q; (void)H_kv; (void)S_q; (void)D; (void)block_size; (void)max_blocks;
+    return 0;
+}
+
+int kf_attn_fwd_paged_q4(const void* Q, const void* cache, const int* block_table, const int* seq_lens, void* O,
+                         float* Mi, float* Li, int B, int H_q, int H_kv, int S_q, int D, int n_blocks, int block_size,
+                         int max_blocks, float scale, unsigned flags, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+    (void)workspace; (void)workspace_bytes;
+    constexpr unsigned known = KF_FLAG_CAUSAL | KF_FLAG_OUT_F16 | KF_FLAG_OUT_BF16 | KF_FLAG_Q_BF16;
+    if ((flags & ~known) || ((flags & KF_FLAG_OUT_F16) && (flags & KF_FLAG_OUT_BF16))) return KF_ERR_INVALID_ARG;
+    if (B < 0 || S_q < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0) return KF_ERR_INVALID_ARG;
+    if (B > 65535 || H_q > 65535) return KF_ERR_INVALID_ARG;
+    if (!q4_dim_ok(D)) return KF_ERR_UNSUPPORTED_HEAD_DIM;
+    if (n_blocks <= 0 || max_blocks <= 0 || !std::isfinite(scale)) return KF_ERR_INVALID_ARG;
+    if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1))) return KF_ERR_INVALID_ARG;
+    if (static_cast<long long>(max_blocks) * block_size >= (1ll << 31)) return KF_ERR_INVALID_ARG;
+    if (static_cast<long long>(H_q / H_kv) * S_q > 64) return KF_ERR_INVALID_ARG;
+    if (B == 0 || S_q == 0) return KF_OK;
+    if (!Q || !cache || !block_table || !seq_lens || !O) return KF_ERR_INVALID_ARG;
+    if (!aligned16(Q) || !aligned16(cache) || !aligned16(O)) return KF_ERR_MISALIGNED;
+    DeviceInfo* di = nullptr;
+    int rc = device_info(&di);
+    if (rc != KF_OK) return rc;
+    kf::Q4AttnParams p;
+    p.cache = static_cast<const uint8_t*>(cache);
+    p.Q = static_cast<const uint16_t*>(Q);
+    p.O = O;
+    p.Mi = Mi;
+    p.Li = Li;
+    p.table = block_table;
+    p.lens = seq_lens;
+    p.B = B;
+    p.H_q = H_q;
+    p.H_kv = H_kv;
+    p.G = H_q / H_kv;
+    p.S_q = S_q;
+    p.n_blocks = n_blocks;
+    p.bs_log2 = log2_exact(block_size);
+    p.max_blocks = max_blocks;
+    p.causal = (flags & KF_FLAG_CAUSAL) != 0;
+    p.q_bf16 = (flags & KF_FLAG_Q_BF16) != 0;
+    p.out_type = (flags & KF_FLAG_OUT_F16) ? kf::KF_OUT_F16 : (flags & KF_FLAG_OUT_BF16) ? kf::KF_OUT_BF16 : kf::KF_OUT_F32;
+    p.scale = scale != 0.f ? scale : 1.0f / std::sqrt(static_cast<float>(D));
+    const unsigned grid = static_cast<unsigned>(B) * H_q * S_q;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (D) {
+        case 64: kf::q4_attn_kernel<64><<<grid, 256, 0, s>>>(p); break;
+        case 128: kf::q4_attn_kernel<128><<<grid, 256, 0, s>>>(p); break;
+        default: kf::q4_attn_kernel<256><<<grid, 256, 0, s>>>(p); break;
+    }
+    return launch_status();
 }
 
 int kf_fill_normal_f16(uint16_t* dst, long long n, unsigned long long seed, long long offset, void* stream) {

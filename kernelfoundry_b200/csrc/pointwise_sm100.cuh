@@ -65,6 +65,17 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
                       pack2<BF16>(f[6], f[7]));
 }
 
+template <bool BF16>
+__device__ __forceinline__ float to_f32(uint16_t u) {
+    if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(u) << 16);
+    return __half2float(__ushort_as_half(u));
+}
+template <bool BF16>
+__device__ __forceinline__ uint16_t from_f32(float x) {
+    if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+    return __half_as_ushort(__float2half_rn(x));
+}
+
 // Rounds 8 fp32 values to the storage type and back.
 template <bool BF16>
 __device__ __forceinline__ void round8(float (&f)[8]) {
@@ -267,6 +278,67 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
                 }
             }
         }
+    }
+}
+
+// ---- Query/key norm with RoPE ---------------------------------------------------
+// y = rnd(rot(x * rsqrt(mean(x^2) + eps) * w)) on every head row of Q and K: one warp per
+// row, the normalised row in shared memory between the norm and the rotation.
+struct QkNormRopeParams {
+    const uint16_t* q;
+    const uint16_t* k;
+    uint16_t* qo;
+    uint16_t* ko;
+    const uint16_t* qw;           // [D], nullptr: ones
+    const uint16_t* kw;
+    const int* pos;               // [B, S] positions, nullptr: position = s
+    const float* inv_freq;        // [rot_dim / 2], nullptr: theta^(-2i/rot_dim)
+    long long q_sb, q_sh, q_ss, k_sb, k_sh, k_ss;        // element strides
+    long long qo_sb, qo_sh, qo_ss, ko_sb, ko_sh, ko_ss;
+    long long n_tokens;           // B * S
+    int S, H_q, H_kv, D, rot_dim;
+    float eps, rot_scale;
+    double log2_theta;
+};
+
+template <bool BF16, bool NEOX>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormRopeParams p) {
+    __shared__ float s_row[8][512];
+    float* y = s_row[threadIdx.x >> 5];
+    const int lane = threadIdx.x & 31;
+    const int H = p.H_q + p.H_kv, half = p.rot_dim / 2;
+    for (long long r = (blockIdx.x * 256ll + threadIdx.x) >> 5; r < p.n_tokens * H; r += gridDim.x * 8ll) {
+        const long long t = r / H;
+        const int h = static_cast<int>(r % H);
+        const long long b = t / p.S, s = t % p.S;
+        const bool is_q = h < p.H_q;
+        const uint16_t* x = is_q ? p.q + b * p.q_sb + h * p.q_sh + s * p.q_ss
+                                 : p.k + b * p.k_sb + (h - p.H_q) * p.k_sh + s * p.k_ss;
+        uint16_t* o = is_q ? p.qo + b * p.qo_sb + h * p.qo_sh + s * p.qo_ss
+                           : p.ko + b * p.ko_sb + (h - p.H_q) * p.ko_sh + s * p.ko_ss;
+        const uint16_t* w = is_q ? p.qw : p.kw;
+        float ss = 0.f;
+        for (int d = lane; d < p.D; d += 32) {
+            y[d] = to_f32<BF16>(x[d]);
+            ss = fmaf(y[d], y[d], ss);
+        }
+        for (int m = 16; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+        const float rinv = rsqrtf(ss / p.D + p.eps);
+        for (int d = lane; d < p.D; d += 32) y[d] *= rinv * (w ? to_f32<BF16>(w[d]) : 1.f);
+        __syncwarp();
+        const int pos = p.pos ? p.pos[t] : static_cast<int>(s);
+        for (int i = lane; i < half; i += 32) {
+            const double f = p.inv_freq ? static_cast<double>(p.inv_freq[i]) : exp2(-(2.0 * i / p.rot_dim) * p.log2_theta);
+            float sn, cs;
+            sincosf(reduce_2pi(pos * f), &sn, &cs);
+            sn *= p.rot_scale;
+            cs *= p.rot_scale;
+            const int i0 = NEOX ? i : 2 * i, i1 = NEOX ? i + half : 2 * i + 1;
+            o[i0] = from_f32<BF16>(fmaf(y[i0], cs, -y[i1] * sn));
+            o[i1] = from_f32<BF16>(fmaf(y[i1], cs, y[i0] * sn));
+        }
+        for (int d = p.rot_dim + lane; d < p.D; d += 32) o[d] = from_f32<BF16>(y[d]);
+        __syncwarp();
     }
 }
 

@@ -1,4 +1,4 @@
-"""Host API of the RMSNorm, RoPE and SwiGLU kernels (include/kf_pointwise.h).
+"""Host API of the RMSNorm, RoPE (alone or with the query/key norm) and SwiGLU kernels (include/kf_pointwise.h).
 
 The reference lists these kernels as planned and has no code for them
 (sviraaj/kernelfoundry, README.md:16-18); the conventions are those of the
@@ -12,9 +12,9 @@ import ctypes
 
 import torch
 
-from ._lib import KF_PW_BF16, KF_ROPE_GPTJ, check, lib
+from ._lib import KF_PW_BF16, KF_ROPE_GPTJ, check, lib, on_device
 
-__all__ = ["rms_norm", "fused_add_rms_norm", "rope_", "swiglu"]
+__all__ = ["rms_norm", "fused_add_rms_norm", "rope_", "qk_norm_rope", "swiglu"]
 
 _DT_FLAGS = {torch.float16: 0, torch.bfloat16: KF_PW_BF16}
 
@@ -127,6 +127,71 @@ def rope_(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor | Non
             raise ValueError("inv_freq must be a contiguous float32 [rot_dim/2] tensor on q's device")
     check(lib().kf_rope(_p(q), _p(k), _p(positions), _p(inv_freq), B, S, H_q, H_kv, D, rot, float(theta),
                         qsb, qsh, qss, ksb, ksh, kss, flags, _stream(q)), "kf_rope")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None,
+                 k_weight: torch.Tensor | None, positions: torch.Tensor | None = None, *, eps: float = 1e-6,
+                 theta: float = 10000.0, rot_dim: int | None = None, interleaved: bool = False,
+                 inv_freq: torch.Tensor | None = None, rot_scale: float = 1.0, layout: str = "bhsd", out=None):
+    """RMSNorm of every head row of ``q`` and ``k`` over D, then the rotary embedding, in one pass.
+
+    ``rnd(rot(x / sqrt(mean(x^2) + eps) * weight))``, rounded once; returns ``(q_out, k_out)``.
+    q ``[B, H_q, S, D]``, k ``[B, H_kv, S, D]`` (``layout="bshd"``: ``[B, S, H, D]``), any
+    strides (multiples of 8) with a contiguous head dimension; ``k`` may be None.  weights
+    ``[D]`` (None: ones).  positions, theta, interleaved, inv_freq as :func:`rope_`;
+    ``rot_dim=0`` norms without rotating; ``rot_scale`` multiplies cos and sin.
+    ``out``: ``(q_out, k_out)`` in ``layout`` to write into -- q and k themselves for in place,
+    or e.g. transposed views to change the storage order.
+    """
+    dev, D = q.device, q.shape[-1]
+    if layout not in ("bhsd", "bshd"):
+        raise ValueError("layout must be 'bhsd' or 'bshd'")
+    if out is None:
+        out = (torch.empty(q.shape, dtype=q.dtype, device=dev),
+               torch.empty(k.shape, dtype=k.dtype, device=dev) if k is not None else None)
+    q_out, k_out = out
+    flag = _DT_FLAGS.get(q.dtype)
+    if flag is None or not q.is_cuda:
+        raise ValueError("tensors must be float16 or bfloat16 CUDA tensors (no CPU path)")
+    s, h = (2, 1) if layout == "bhsd" else (1, 2)
+    strides, heads = [], []
+    for x, y in ((q, q_out), (k, k_out)):
+        if x is None:
+            if y is not None:
+                raise ValueError("k_out without k")
+            heads.append(0)
+            strides += [0] * 6
+            continue
+        for t in (x, y):
+            if t is None or t.dtype != q.dtype or t.device != dev or t.dim() != 4 or t.stride(3) != 1:
+                raise ValueError("q, k and out must be 4-D tensors of one type and device with a contiguous head dimension")
+        if y.shape != x.shape or x.shape[0] != q.shape[0] or x.shape[s] != q.shape[s] or x.shape[3] != D:
+            raise ValueError("k must match q in B, S and D, and out q and k")
+        heads.append(x.shape[h])
+        for t in (x, y):
+            st = t.stride()
+            strides += [st[0], st[h], st[s]]
+    B, S = q.shape[0], q.shape[s]
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != q.dtype or w.device != dev or w.dim() != 1 or w.shape[0] != D
+                              or not w.is_contiguous()):
+            raise ValueError("weights must be contiguous [D] tensors of q's type and device")
+    rot = D if rot_dim is None else int(rot_dim)
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (B, S)
+                                  or not positions.is_contiguous() or positions.device != dev):
+        raise ValueError("positions must be a contiguous int32 [B, S] tensor on q's device")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2
+                                 or not inv_freq.is_contiguous() or inv_freq.device != dev):
+        raise ValueError("inv_freq must be a contiguous float32 [rot_dim/2] tensor on q's device")
+    qi, qo, ki, ko = strides[0:3], strides[3:6], strides[6:9], strides[9:12]
+
+    def ptr(t):
+        return t.data_ptr() if t is not None else None
+
+    on_device(dev.index, lib().kf_qk_norm_rope, "kf_qk_norm_rope", q.data_ptr(), ptr(k), ptr(q_weight), ptr(k_weight),
+              q_out.data_ptr(), ptr(k_out), ptr(positions), ptr(inv_freq), B, S, heads[0], heads[1], D, rot,
+              theta, rot_scale, eps, *qi, *ki, *qo, *ko, flag | (KF_ROPE_GPTJ if interleaved else 0))
+    return q_out, k_out
 
 
 def swiglu(gate_up: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
