@@ -1512,6 +1512,33 @@ int log2_exact(int v) {
     return l;
 }
 
+// ---- attention over it
+constexpr int kQ4MaxRows = 64;                // query rows of one cache head in a call
+
+// 8-row query tiles a warp carries: two where the accumulators (MT * 4 * NT registers) fit.
+int q4_attn_nt(int D, int R) { return R > 8 && D <= 128 ? 2 : 1; }
+
+size_t q4_attn_part_bytes(int D, int R) {
+    const int rows = 8 * q4_attn_nt(D, R);
+    return static_cast<size_t>(rows) * (D + 2) * sizeof(float);
+}
+
+// Tickets at the head of the workspace (shared with the decode kernel's), two parts per CTA after them.
+size_t q4_attn_ws_bytes(int D, int R, int sm_count) { return kCounterBytes + q4_attn_part_bytes(D, R) * 2 * sm_count; }
+
+template <int D, int NT>
+int q4_attn_launch(const kf::Q4AttnParams& p, long long max_tiles, int sm_count, cudaStream_t s) {
+    using C = kf::Q4AttnCfg<D, NT>;
+    static_assert(C::PART_FLOATS == 8 * NT * (D + 2), "part size");
+    int bps = 0;
+    const int rc = kernel_setup<kf::q4_attn_kernel<D, NT>>(C::SMEM_BYTES, C::THREADS, &bps);
+    if (rc != KF_OK) return rc;
+    const long long want = (max_tiles + C::W - 1) / C::W;
+    const unsigned grid = static_cast<unsigned>(want < sm_count ? want : sm_count);
+    const cudaError_t e = launch_pdl(kf::q4_attn_kernel<D, NT>, dim3(grid), C::THREADS, C::SMEM_BYTES, s, p);
+    return e == cudaSuccess ? KF_OK : cuda_fail(e);
+}
+
 int q4_io_params(const void* cache, const int* slots, const void* k, const void* v, int B, int S, int H_kv, int D,
                  int n_blocks, int block_size, long long ksb, long long ksh, long long kss, long long vsb,
                  long long vsh, long long vss, unsigned flags, kf::Q4IoParams* p) {
@@ -1586,15 +1613,18 @@ int kf_kv_read_q4(const void* cache, const int* slots, void* k, void* v, int B, 
 }
 
 size_t kf_attn_paged_q4_workspace_bytes(int B, int H_q, int H_kv, int S_q, int D, int block_size, int max_blocks) {
-    (void)B; (void)H_q; (void)H_kv; (void)S_q; (void)D; (void)block_size; (void)max_blocks;
-    return 0;
+    if (B <= 0 || S_q <= 0 || H_kv <= 0 || H_q <= 0 || H_q % H_kv != 0 || !q4_dim_ok(D)) return 0;
+    if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1)) || max_blocks <= 0) return 0;
+    const long long R = static_cast<long long>(H_q / H_kv) * S_q;
+    DeviceInfo* di = nullptr;
+    if (R > kQ4MaxRows || device_info(&di) != KF_OK) return 0;
+    return q4_attn_ws_bytes(D, static_cast<int>(R), di->sm_count);
 }
 
 int kf_attn_fwd_paged_q4(const void* Q, const void* cache, const int* block_table, const int* seq_lens, void* O,
                          float* Mi, float* Li, int B, int H_q, int H_kv, int S_q, int D, int n_blocks, int block_size,
                          int max_blocks, float scale, unsigned flags, void* workspace, size_t workspace_bytes,
                          void* stream) {
-    (void)workspace; (void)workspace_bytes;
     constexpr unsigned known = KF_FLAG_CAUSAL | KF_FLAG_OUT_F16 | KF_FLAG_OUT_BF16 | KF_FLAG_Q_BF16;
     if ((flags & ~known) || ((flags & KF_FLAG_OUT_F16) && (flags & KF_FLAG_OUT_BF16))) return KF_ERR_INVALID_ARG;
     if (B < 0 || S_q < 0 || H_q <= 0 || H_kv <= 0 || H_q % H_kv != 0) return KF_ERR_INVALID_ARG;
@@ -1602,14 +1632,20 @@ int kf_attn_fwd_paged_q4(const void* Q, const void* cache, const int* block_tabl
     if (!q4_dim_ok(D)) return KF_ERR_UNSUPPORTED_HEAD_DIM;
     if (n_blocks <= 0 || max_blocks <= 0 || !std::isfinite(scale)) return KF_ERR_INVALID_ARG;
     if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1))) return KF_ERR_INVALID_ARG;
-    if (static_cast<long long>(max_blocks) * block_size >= (1ll << 31)) return KF_ERR_INVALID_ARG;
-    if (static_cast<long long>(H_q / H_kv) * S_q > 64) return KF_ERR_INVALID_ARG;
+    const long long keys = static_cast<long long>(max_blocks) * block_size;
+    const long long R = static_cast<long long>(H_q / H_kv) * S_q;
+    if (keys >= (1ll << 31) || R > kQ4MaxRows) return KF_ERR_INVALID_ARG;
     if (B == 0 || S_q == 0) return KF_OK;
     if (!Q || !cache || !block_table || !seq_lens || !O) return KF_ERR_INVALID_ARG;
-    if (!aligned16(Q) || !aligned16(cache) || !aligned16(O)) return KF_ERR_MISALIGNED;
+    if (!aligned16(Q) || !aligned16(cache) || !aligned16(O) || !aligned16(workspace)) return KF_ERR_MISALIGNED;
+    const int nt = q4_attn_nt(D, static_cast<int>(R));
+    const int n_rg = static_cast<int>((R + 8 * nt - 1) / (8 * nt));
+    const long long tiles = static_cast<long long>(B) * H_kv * n_rg * ((keys + 31) / 32);   // an upper bound
+    if (tiles >= (1ll << 31)) return KF_ERR_INVALID_ARG;
     DeviceInfo* di = nullptr;
     int rc = device_info(&di);
     if (rc != KF_OK) return rc;
+    if (!workspace || workspace_bytes < q4_attn_ws_bytes(D, static_cast<int>(R), di->sm_count)) return KF_ERR_WORKSPACE;
     kf::Q4AttnParams p;
     p.cache = static_cast<const uint8_t*>(cache);
     p.Q = static_cast<const uint16_t*>(Q);
@@ -1618,26 +1654,27 @@ int kf_attn_fwd_paged_q4(const void* Q, const void* cache, const int* block_tabl
     p.Li = Li;
     p.table = block_table;
     p.lens = seq_lens;
+    p.tickets = static_cast<unsigned*>(workspace);
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
     p.B = B;
-    p.H_q = H_q;
     p.H_kv = H_kv;
-    p.G = H_q / H_kv;
     p.S_q = S_q;
+    p.R = static_cast<int>(R);
+    p.n_rg = n_rg;
     p.n_blocks = n_blocks;
     p.bs_log2 = log2_exact(block_size);
     p.max_blocks = max_blocks;
     p.causal = (flags & KF_FLAG_CAUSAL) != 0;
     p.q_bf16 = (flags & KF_FLAG_Q_BF16) != 0;
     p.out_type = (flags & KF_FLAG_OUT_F16) ? kf::KF_OUT_F16 : (flags & KF_FLAG_OUT_BF16) ? kf::KF_OUT_BF16 : kf::KF_OUT_F32;
-    p.scale = scale != 0.f ? scale : 1.0f / std::sqrt(static_cast<float>(D));
-    const unsigned grid = static_cast<unsigned>(B) * H_q * S_q;
+    p.scale_log2 = (scale != 0.f ? scale : 1.0f / std::sqrt(static_cast<float>(D))) * 1.4426950408889634f;
+    p.timeout_ns = g_timeout_ns.load();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (D) {
-        case 64: kf::q4_attn_kernel<64><<<grid, 256, 0, s>>>(p); break;
-        case 128: kf::q4_attn_kernel<128><<<grid, 256, 0, s>>>(p); break;
-        default: kf::q4_attn_kernel<256><<<grid, 256, 0, s>>>(p); break;
+        case 64: return nt == 1 ? q4_attn_launch<64, 1>(p, tiles, di->sm_count, s) : q4_attn_launch<64, 2>(p, tiles, di->sm_count, s);
+        case 128: return nt == 1 ? q4_attn_launch<128, 1>(p, tiles, di->sm_count, s) : q4_attn_launch<128, 2>(p, tiles, di->sm_count, s);
+        default: return q4_attn_launch<256, 1>(p, tiles, di->sm_count, s);
     }
-    return launch_status();
 }
 
 int kf_fill_normal_f16(uint16_t* dst, long long n, unsigned long long seed, long long offset, void* stream) {
