@@ -19,8 +19,11 @@
 // Queries are scaled by a power of two per row to a maximum in [2^13, 2^14), which holds fp16
 // rows exactly, and bf16 ones but for elements below 2^-28 of the row's largest.
 // p t enters the second product as fp16, scaled by a power of two such that the largest t seen
-// is below 2^14 (t spans any range; small ones lose bits only against the largest).  This
+// stays below 2^7 (t spans any range; small ones lose bits only against the largest).  This
 // rounding, 2^-11 relative per key, is the only one below fp32 in the sum.
+// The running maximum is lazy: p = 2^(x - m) with an m that is raised only when a score passes
+// m + 8 (p <= 2^8 then, which fp16 and fp32 hold as well as p <= 1), so a tile needs one vote
+// instead of a maximum across the warp.  The true maximum is kept per thread and put in at the end.
 //
 // Work split.  Every (sequence, cache head, group of 8 NT query rows) is a unit of 32-key
 // tiles; all units' tiles in a row are cut evenly over the CTAs (one per SM) and each CTA's
@@ -109,19 +112,30 @@ __device__ __forceinline__ void q4_unpack4(uint32_t x, uint32_t negz, uint32_t (
 
 // A warp's position in the row of tiles.
 struct Q4Cursor {
-    int b, hr, tile, nt, len;
+    int b, h, rg, tile;            // sequence, cache head, row group, tile of 32 keys
+    int nt, len;                   // the sequence's tiles and keys
 };
 
 template <int D, int NT>
-struct Q4Warp {                    // a warp's running state of one unit
+struct Q4Warp {                    // a warp's running state of one unit; pairs: columns 2t, 2t + 1
     float o[NT][Q4AttnCfg<D, NT>::MT][4];
-    float m[NT][2], ms[NT][2], l[NT][2];       // ms: m, or 0 while m is -inf
+    float2 m[NT], ms[NT], l[NT];   // reference of the exponent (ms: 0 while it is -inf), sum of p
+    float2 mt[NT];                 // this thread's largest score
     uint32_t q[NT][Q4AttnCfg<D, NT>::KW][4];
-    float cq[NT][2];               // a column's factor of the scores
+    float2 cq[NT];                 // a column's factor of the scores
     int lim[NT][2];                // keys the column's query sees
-    uint32_t tmax;                 // bits of the largest value scale seen
-    float tnorm, tinv;             // 2^13 / 2^exponent(tmax), and its inverse
+    float tlim, tnorm, tinv;       // value scales up to tlim times tnorm stay below 2^7; tinv = 1 / tnorm
 };
+
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fmax2(float2 a, float2 b) { return make_float2(fmaxf(a.x, b.x), fmaxf(a.y, b.y)); }
 
 __device__ __forceinline__ int q4_len(const Q4AttnParams& p, int b) {
     const int cap = p.max_blocks << p.bs_log2;
@@ -131,37 +145,55 @@ __device__ __forceinline__ int q4_len(const Q4AttnParams& p, int b) {
 // Tiles of a sequence: an empty one keeps one (masked) tile, whose unit writes the zeros.
 __device__ __forceinline__ int q4_tiles(int len) { return len <= 32 ? 1 : (len + 31) >> 5; }
 
-__device__ __forceinline__ void q4_advance(const Q4AttnParams& p, Q4Cursor& c, int HR) {
+__device__ __forceinline__ void q4_advance(const Q4AttnParams& p, Q4Cursor& c) {
     if (++c.tile < c.nt) return;
     c.tile = 0;
-    if (++c.hr < HR) return;
-    c.hr = 0;
+    if (++c.rg < p.n_rg) return;
+    c.rg = 0;
+    if (++c.h < p.H_kv) return;
+    c.h = 0;
     if (++c.b < p.B) {
         c.len = q4_len(p, c.b);
         c.nt = q4_tiles(c.len);
     }
 }
+__device__ __forceinline__ int q4_unit(const Q4AttnParams& p, const Q4Cursor& c) {
+    return (c.b * p.H_kv + c.h) * p.n_rg + c.rg;
+}
 
-// Unit start: queries to MMA operands (B fragments: column = query g, k = dims of lane t).
+// The unit's query rows, raw (lane (g, t): row g of each 8, its chunks of 8 dims).
 template <int D, int NT>
-__device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s, const Q4Cursor& c, int lane) {
+__device__ __forceinline__ void q4_load_q(const Q4AttnParams& p, uint4 (&raw)[NT][Q4AttnCfg<D, NT>::KW], const Q4Cursor& c,
+                                          int lane) {
     using C = Q4AttnCfg<D, NT>;
     const int g = lane >> 2, t = lane & 3;
-    const int h = c.hr / p.n_rg, row0 = (c.hr % p.n_rg) * C::ROWS;
-    const size_t qbase = (static_cast<size_t>(c.b) * p.H_kv + h) * p.R;
-    s.tmax = 0u;
-    s.tnorm = s.tinv = 1.0f;
+    const uint16_t* q = p.Q + (static_cast<size_t>(c.b) * p.H_kv + c.h) * p.R * D;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = row0 + 8 * n + g;
-        float x[C::KW][8], mx = 0.f;
+        const int r = c.rg * C::ROWS + 8 * n + g;
 #pragma unroll
         for (int i = 0; i < C::KW; ++i) {
             const int chunk = D == 64 ? 2 * t + i : (i >> 2) * 16 + 4 * t + (i & 3);
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (r < p.R) v = reinterpret_cast<const uint4*>(p.Q + (qbase + r) * D)[chunk];
-            if (p.q_bf16) unpack8<true>(v, x[i]);
-            else unpack8<false>(v, x[i]);
+            raw[n][i] = r < p.R ? reinterpret_cast<const uint4*>(q + static_cast<size_t>(r) * D)[chunk] : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+}
+
+// Unit start: queries to MMA operands (B fragments: column = query g, k = dims of lane t).
+template <int D, int NT>
+__device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s, const uint4 (&raw)[NT][Q4AttnCfg<D, NT>::KW],
+                                         const Q4Cursor& c, int lane) {
+    using C = Q4AttnCfg<D, NT>;
+    const int t = lane & 3;
+    s.tlim = 0.f;
+    s.tnorm = s.tinv = 1.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float x[C::KW][8], mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < C::KW; ++i) {
+            if (p.q_bf16) unpack8<true>(raw[n][i], x[i]);
+            else unpack8<false>(raw[n][i], x[i]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
         }
@@ -171,20 +203,17 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
         ex = ex < 14 ? 14 : ex;
         const float f = __uint_as_float(static_cast<uint32_t>(267 - ex) << 23);   // 2^13 / 2^(ex - 127)
 #pragma unroll
-        for (int i = 0; i < C::KW; ++i) {
+        for (int i = 0; i < C::KW; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s.q[n][i][e] = pack_half2(x[i][e] * f, x[i][e + 4] * f);
-        }
         const float cq = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(ex - 13) << 23) * 0x1p9f;
+        s.cq[n].x = __shfl_sync(0xffffffffu, cq, 8 * t);
+        s.cq[n].y = __shfl_sync(0xffffffffu, cq, 8 * t + 4);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            s.cq[n][k] = __shfl_sync(0xffffffffu, cq, 4 * (2 * t + k));
-            const int i = (row0 + 8 * n + 2 * t + k) % p.S_q;
-            s.lim[n][k] = c.len - (p.causal ? p.S_q - 1 - i : 0);
-            s.m[n][k] = -INFINITY;
-            s.ms[n][k] = 0.f;
-            s.l[n][k] = 0.f;
-        }
+        for (int k = 0; k < 2; ++k)
+            s.lim[n][k] = c.len - (p.causal ? p.S_q - 1 - (c.rg * C::ROWS + 8 * n + 2 * t + k) % p.S_q : 0);
+        s.m[n] = s.mt[n] = make_float2(-INFINITY, -INFINITY);
+        s.ms[n] = s.l[n] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < C::MT; ++i)
 #pragma unroll
@@ -192,17 +221,15 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
     }
 }
 
-// One tile of 32 keys from shared memory.  valid: bit j set when group j was copied.
-template <int D, int NT>
-__device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s, const uint8_t* st, int key0, int len,
-                                        uint32_t valid, bool masked, int lane) {
+// One tile of 32 keys from shared memory.  MASKED: some key is outside the sequence, hidden
+// from a row, or in a page outside the pool (valid: bit j set when group j was copied).
+template <int D, int NT, bool MASKED>
+__device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int key0, int len, uint32_t valid, int lane) {
     using C = Q4AttnCfg<D, NT>;
     const int g = lane >> 2, t = lane & 3;
-    float x[2][NT][4], mx[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
-    // S^T = K Q^T.  Every word of 8 dims has its own accumulator (the chains of two MMAs do not
-    // wait on one another), added up in fp32.
+    float2 x[2][NT][2];            // scores [group][query tile][row g or g + 8]
+    float tv[2][2];                // value scales of the same rows
+    // S^T = K Q^T, in two chains per 128 dims, added up in fp32
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const uint8_t* gr = st + j * C::GROUP;
@@ -223,7 +250,11 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
                 wa[0] = a.x; wa[1] = a.y; wa[2] = a.z; wa[3] = a.w;
                 wb[0] = b.x; wb[1] = b.y; wb[2] = b.z; wb[3] = b.w;
             }
-            float acc[NW][NT][4];
+            float acc[2][NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[0][n][e] = acc[1][n][e] = 0.f;
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 const int w = hf * 4 + i;
@@ -232,89 +263,84 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
                 const uint32_t c0 = q4_lo(ua, za), c1 = q4_lo(ub, zb), c2 = q4_hi(ua, za), c3 = q4_hi(ub, zb);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
-                    mma_16816(acc[i][n], a0, a1, a2, a3, s.q[n][w][0], s.q[n][w][1]);
-                    mma_16816(acc[i][n], c0, c1, c2, c3, s.q[n][w][2], s.q[n][w][3]);
+                    mma_16816(acc[0][n], a0, a1, a2, a3, s.q[n][w][0], s.q[n][w][1]);
+                    mma_16816(acc[1][n], c0, c1, c2, c3, s.q[n][w][2], s.q[n][w][3]);
                 }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = acc[0][n][e] + acc[1][n][e];
-                    if constexpr (NW == 4) v += acc[2][n][e] + acc[3][n][e];
-                    x[j][n][e] = hf == 0 ? v : x[j][n][e] + v;
+                for (int h = 0; h < 2; ++h) {
+                    const float2 v = fadd2(make_float2(acc[0][n][2 * h], acc[0][n][2 * h + 1]),
+                                           make_float2(acc[1][n][2 * h], acc[1][n][2 * h + 1]));
+                    x[j][n][h] = hf == 0 ? v : fadd2(x[j][n][h], v);
                 }
         }
-        // Scores, masks and the tile's maxima (rows g and g + 8; columns 2t, 2t + 1).
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            const int key = key0 + 16 * j + 8 * h + g;
             const float sc = q4_scale(wk[h]);
+            tv[j][h] = q4_scale(words[16 + g + 8 * h]);
+            if (MASKED && (!((valid >> j) & 1u) || key >= len)) tv[j][h] = 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    float v = x[j][n][2 * h + k] * (sc * s.cq[n][k]);
-                    if (masked) {
-                        if (!((valid >> j) & 1u)) v = 0.f;               // a page outside the pool reads zeros
-                        if (key0 + 16 * j + 8 * h + g >= s.lim[n][k]) v = -INFINITY;
-                    }
-                    x[j][n][2 * h + k] = v;
-                    mx[n][k] = fmaxf(mx[n][k], v);
+            for (int n = 0; n < NT; ++n) {
+                float2 v = fmul2(x[j][n][h], fmul2(make_float2(sc, sc), s.cq[n]));
+                if (MASKED) {
+                    if (!((valid >> j) & 1u)) v = make_float2(0.f, 0.f);     // a page outside the pool reads zeros
+                    if (key >= s.lim[n][0]) v.x = -INFINITY;
+                    if (key >= s.lim[n][1]) v.y = -INFINITY;
                 }
+                x[j][n][h] = v;
+            }
         }
     }
-    // The largest value scale so far sets the fp16 range of p t.
-    {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(st + (lane >> 4) * C::GROUP + Q4<D>::V_WORDS);
-        uint32_t u = words[lane & 15] & 0xFFFFFF00u;
-        if (u >= 0x7F800000u) u = 0u;                                    // a spoiled row sets no range
-        if (masked && (!((valid >> (lane >> 4)) & 1u) || key0 + lane >= len)) u = 0u;
-        u = __reduce_max_sync(0xffffffffu, u);
-        if (u > s.tmax) {
-            s.tmax = u;
-            int ex = static_cast<int>(u >> 23);
-            ex = ex < 27 ? 27 : ex;                                      // scales are 0 or at least 2^-100
-            const float norm = __uint_as_float(static_cast<uint32_t>(267 - ex) << 23);
-            const float r = norm * s.tinv;
-            s.tnorm = norm;
-            s.tinv = __uint_as_float(static_cast<uint32_t>(ex - 13) << 23);
+    // Does a score pass m + 8, or a value scale the range of p t?  Rarely.
+    float2 mx[NT];
+    const float tm = fmaxf(fmaxf(tv[0][0], tv[0][1]), fmaxf(tv[1][0], tv[1][1]));   // (a spoiled row's NaN is ignored)
+    bool up = tm > s.tlim;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < C::MT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s.o[n][i][e] *= r;
-        }
+    for (int n = 0; n < NT; ++n) {
+        mx[n] = fmax2(fmax2(x[0][n][0], x[0][n][1]), fmax2(x[1][n][0], x[1][n][1]));
+        s.mt[n] = fmax2(s.mt[n], mx[n]);
+        up = up || mx[n].x > s.m[n].x + 8.0f || mx[n].y > s.m[n].y + 8.0f;
     }
-    bool grew = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            mx[n][k] = fmaxf(mx[n][k], __shfl_xor_sync(0xffffffffu, mx[n][k], 4));
-            mx[n][k] = fmaxf(mx[n][k], __shfl_xor_sync(0xffffffffu, mx[n][k], 8));
-            mx[n][k] = fmaxf(mx[n][k], __shfl_xor_sync(0xffffffffu, mx[n][k], 16));
-            grew = grew || mx[n][k] > s.m[n][k];
+    if (__any_sync(0xffffffffu, up)) {
+        const float tt = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(tm, 0.f))));
+        float r = 1.0f;
+        if (tt > s.tlim) {
+            int e = static_cast<int>(__float_as_uint(tt) >> 23);             // 27 or more: scales are 0 or >= 2^-100
+            e = e < 7 ? 7 : e;                                               // (but the bytes are the caller's)
+            s.tlim = __uint_as_float(static_cast<uint32_t>(e < 254 ? e + 1 : 254) << 23);
+            s.tnorm = __uint_as_float(static_cast<uint32_t>(260 - e) << 23);  // 2^6 / 2^(e - 127)
+            r = s.tnorm * s.tinv;
+            s.tinv = __uint_as_float(static_cast<uint32_t>(e - 6) << 23);
         }
-    if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+            float v[2] = {mx[n].x, mx[n].y}, a[2];
+            float m[2] = {s.m[n].x, s.m[n].y}, ms[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float m = fmaxf(s.m[n][k], mx[n][k]);
-                const float ms = m == -INFINITY ? 0.f : m;
-                const float a = ex2_approx(s.m[n][k] - ms);
-                s.m[n][k] = m;
-                s.ms[n][k] = ms;
-                s.l[n][k] *= a;
-#pragma unroll
-                for (int i = 0; i < C::MT; ++i) {
-                    s.o[n][i][k] *= a;
-                    s.o[n][i][2 + k] *= a;
-                }
+                v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 4));
+                v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 8));
+                v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 16));
+                v[k] = fmaxf(v[k], m[k]);
+                ms[k] = v[k] == -INFINITY ? 0.f : v[k];
+                a[k] = ex2_approx(m[k] - ms[k]);
             }
+            s.m[n] = make_float2(v[0], v[1]);
+            s.ms[n] = make_float2(ms[0], ms[1]);
+            s.l[n] = make_float2(s.l[n].x * a[0], s.l[n].y * a[1]);
+            a[0] *= r;
+            a[1] *= r;
+#pragma unroll
+            for (int i = 0; i < C::MT; ++i) {
+                s.o[n][i][0] *= a[0];
+                s.o[n][i][1] *= a[1];
+                s.o[n][i][2] *= a[0];
+                s.o[n][i][3] *= a[1];
+            }
+        }
     }
     // O^T += V^T P^T
 #pragma unroll
@@ -324,24 +350,25 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
         uint32_t pb[NT][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float tv = q4_scale(words[g + 8 * h]) * s.tnorm;
-            if (masked && (!((valid >> j) & 1u) || key0 + 16 * j + 8 * h + g >= len)) tv = 0.f;
+            const float tn = tv[j][h] * s.tnorm;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float pt[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float pr = ex2_approx(x[j][n][2 * h + k] - s.ms[n][k]);
-                    s.l[n][k] += pr;
-                    pt[k] = pr * tv;
-                    if (masked && key0 + 16 * j + 8 * h + g >= s.lim[n][k]) pt[k] = 0.f;   // 0 * a spoiled row's NaN
+                const float2 d = fadd2(x[j][n][h], make_float2(-s.ms[n].x, -s.ms[n].y));
+                const float2 pr = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+                s.l[n] = fadd2(s.l[n], pr);
+                float2 pt = fmul2(pr, make_float2(tn, tn));
+                if (MASKED) {                                                // 0 * a spoiled row's NaN
+                    const int key = key0 + 16 * j + 8 * h + g;
+                    if (key >= s.lim[n][0]) pt.x = 0.f;
+                    if (key >= s.lim[n][1]) pt.y = 0.f;
                 }
-                pb[n][h] = movmatrix_trans(pack_half2(pt[0], pt[1]));
+                pb[n][h] = movmatrix_trans(pack_half2(pt.x, pt.y));
             }
         }
         const uint2 z01 = *reinterpret_cast<const uint2*>(words + 2 * t);
         const uint2 z89 = *reinterpret_cast<const uint2*>(words + 8 + 2 * t);
-        const uint32_t za = q4_negz((z01.x & 15u) | ((z01.y & 15u) << 16)), zb = q4_negz((z89.x & 15u) | ((z89.y & 15u) << 16));
+        const uint32_t za = q4_negz(__byte_perm(z01.x, z01.y, 0x5410) & kNibLo);
+        const uint32_t zb = q4_negz(__byte_perm(z89.x, z89.y, 0x5410) & kNibLo);
         const uint8_t* vr = gr + Q4<D>::V_CODES + 2 * t * (D / 2);
         constexpr int R1 = D / 2, R8 = 8 * (D / 2);                      // next key, eighth next key
         if constexpr (D == 64) {
@@ -401,22 +428,27 @@ struct Q4Unit {
 
 // End of a warp's share of a unit: O, m and l in true units, to the output or to a part.
 template <int D, int NT>
-__device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s, int u, bool whole, float* part, int lane) {
+__device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s, const Q4Cursor& c, bool whole, float* part,
+                                        int lane) {
     using C = Q4AttnCfg<D, NT>;
     const int g = lane >> 2, t = lane & 3;
-    const int row0 = (u % p.n_rg) * C::ROWS;
-    const size_t rbase = static_cast<size_t>(u / p.n_rg) * p.R;
+    const int row0 = c.rg * C::ROWS;
+    const size_t rbase = (static_cast<size_t>(c.b) * p.H_kv + c.h) * p.R;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            float l = s.l[n][k];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            float l = k ? s.l[n].y : s.l[n].x, m = k ? s.mt[n].y : s.mt[n].x;
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                l += __shfl_xor_sync(0xffffffffu, l, o);
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            }
+            // From the exponent's reference to the true maximum (at most 8 above it).
+            const float a = m == -INFINITY ? 1.0f : ex2_approx((k ? s.m[n].y : s.m[n].x) - m);
+            l *= a;
             const int col = 8 * n + 2 * t + k, r = row0 + col;
-            // 2^9 first: with the scales' power in one factor it could leave fp32's range
-            const float f = whole ? s.tinv * (l == 0.f ? 0.f : 1.0f / l) : s.tinv;
+            const float f = whole ? s.tinv * a * (l == 0.f ? 0.f : 1.0f / l) : s.tinv * a;
 #pragma unroll
             for (int set = 0; set < C::SETS; ++set)
 #pragma unroll
@@ -425,8 +457,7 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
                     for (int v = 0; v < C::V4; ++v) {
                         float y[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            y[i] = s.o[n][set * 8 + 4 * v + i][2 * h + k] * 0x1p9f * f;
+                        for (int i = 0; i < 4; ++i) y[i] = s.o[n][set * 8 + 4 * v + i][2 * h + k] * 0x1p9f * f;
                         const float4 y4 = make_float4(y[0], y[1], y[2], y[3]);
                         const int e = 2 * h + k;
                         if (!whole)
@@ -436,10 +467,10 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
                     }
             if (g == 0) {
                 if (!whole) {
-                    part[C::O_FLOATS + col] = s.m[n][k];
+                    part[C::O_FLOATS + col] = m;
                     part[C::O_FLOATS + C::ROWS + col] = l;
                 } else if (r < p.R) {
-                    if (p.Mi) p.Mi[rbase + r] = s.m[n][k] * 0.6931471805599453f;
+                    if (p.Mi) p.Mi[rbase + r] = m * 0.6931471805599453f;
                     if (p.Li) p.Li[rbase + r] = l;
                 }
             }
@@ -458,6 +489,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     __shared__ int s_sum[W];
     __shared__ int s_b[W], s_base[W];
     __shared__ Q4Unit s_ent[2 * W];
+    __shared__ float s_wt[2 * W][C::ROWS], s_mx[2 * W][C::ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* heads = reinterpret_cast<float*>(smem + C::RING_BYTES);
     uint8_t* ring = smem + warp * STAGES * C::STAGE_BYTES;
@@ -485,81 +517,101 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     }
     if (lane == 31) s_sum[warp] = incl;
     __syncthreads();
-    int total = 0, before = incl - mine;
+    unsigned total = 0, before = incl - mine;
+#pragma unroll
     for (int w = 0; w < W; ++w) {
-        before += w < warp ? s_sum[w] : 0;
-        total += s_sum[w];
+        const unsigned v = s_sum[w];
+        before += w < warp ? v : 0u;
+        total += v;
     }
-    const long long T = static_cast<long long>(total) * HR;
-    // CTAs that take part: every warp of theirs gets at least a tile.
-    long long act = (T + W - 1) / W;
-    if (act > gridDim.x) act = gridDim.x;
+    const unsigned T = total * HR;                                       // < 2^31, the host sees to it
+    // CTAs that take part: every warp of theirs gets at least a tile.  CTA c has the tiles from
+    // c * quot + min(c, rem), warp w of it those from x0 + w * (x1 - x0) / W.
+    const unsigned want = (T + W - 1) / W, act = want < gridDim.x ? want : gridDim.x;
     if (blockIdx.x >= act) return;
-    const long long x0 = blockIdx.x * T / act, x1 = (blockIdx.x + 1) * T / act;
+    const unsigned quot = T / act, rem = T - quot * act;
+    const int x0 = blockIdx.x * quot + (blockIdx.x < rem ? blockIdx.x : rem), x1 = x0 + quot + (blockIdx.x < rem ? 1 : 0);
+    const int wq = (x1 - x0) / W, wr = (x1 - x0) % W;
+    auto warp_start = [&](int w) { return x0 + w * wq + (w < wr ? w : wr); };
     if (mine > 0) {
-        const long long lo = static_cast<long long>(before) * HR, hi = lo + static_cast<long long>(mine) * HR;
-        for (int w = 0; w < W; ++w) {
-            const long long y = x0 + w * (x1 - x0) / W;
-            if (y >= lo && y < hi) {
-                long long at = lo;
-                int b = b0;
+        const int lo = before * HR, hi = lo + mine * HR;
+        if (hi > x0 && lo < x1)
+            for (int w = 0; w < W; ++w) {
+                const int y = warp_start(w);
+                if (y < lo || y >= hi) continue;
+                int at = lo, b = b0;
                 for (; b < b1 - 1; ++b) {
-                    const long long next = at + static_cast<long long>(q4_tiles(q4_len(p, b))) * HR;
+                    const int next = at + q4_tiles(q4_len(p, b)) * HR;
                     if (y < next) break;
                     at = next;
                 }
                 s_b[w] = b;
-                s_base[w] = static_cast<int>(at);
+                s_base[w] = at;
             }
-        }
     }
     __syncthreads();
 
-    const int y0 = static_cast<int>(x0 + warp * (x1 - x0) / W), y1 = static_cast<int>(x0 + (warp + 1) * (x1 - x0) / W);
+    const int y0 = warp_start(warp), y1 = warp_start(warp + 1);
     if (y0 < y1) {
         Q4Cursor cur;
         cur.b = s_b[warp];
         cur.len = q4_len(p, cur.b);
         cur.nt = q4_tiles(cur.len);
-        cur.hr = (y0 - s_base[warp]) / cur.nt;
-        cur.tile = (y0 - s_base[warp]) % cur.nt;
+        {
+            const unsigned off = y0 - s_base[warp], hr = off / cur.nt;
+            cur.tile = off - hr * cur.nt;
+            cur.h = hr;
+            cur.rg = 0;
+            if (p.n_rg > 1) {
+                cur.h = hr / p.n_rg;
+                cur.rg = hr - cur.h * p.n_rg;
+            }
+        }
         Q4Cursor pre = cur;                                              // next tile to copy
         int win = -1, win_b = -1, win_p = 0;                             // 32 table entries, one per lane
         uint32_t vbits = 0;                                              // 2 validity bits per stage
-        const size_t page_bytes = static_cast<size_t>(C::GROUP) << (p.bs_log2 - 4);
+        const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
+        const bool paired = p.bs_log2 == 4;                              // a group is a page: a tile takes two copies
 
         auto copy = [&](int stage) {
             const int key0 = pre.tile * 32, rem = pre.len - key0;
             const int ng = rem <= 0 ? 0 : rem <= 16 ? 1 : 2;
-            const int p0 = key0 >> p.bs_log2, p1 = p.bs_log2 == 4 && ng == 2 ? p0 + 1 : p0;
-            if (ng && (pre.b != win_b || p0 < win_p || p1 >= win_p + 32)) {
+            const int p0 = key0 >> p.bs_log2;
+            if (ng && (pre.b != win_b || static_cast<unsigned>(p0 - win_p) >= 31u)) {
                 win_b = pre.b;
                 win_p = p0;
                 const int used = (pre.len + (1 << p.bs_log2) - 1) >> p.bs_log2;
                 win = p0 + lane < used ? p.table[static_cast<size_t>(pre.b) * p.max_blocks + p0 + lane] : -1;
             }
-            const int e0 = __shfl_sync(0xffffffffu, win, (p0 - win_p) & 31);
-            const int e1 = __shfl_sync(0xffffffffu, win, (p1 - win_p) & 31);
+            const int e0 = __shfl_sync(0xffffffffu, win, p0 - win_p);
+            const int e1 = paired ? __shfl_sync(0xffffffffu, win, p0 - win_p + 1) : e0;
             const bool v0 = ng >= 1 && static_cast<unsigned>(e0) < static_cast<unsigned>(p.n_blocks);
             const bool v1 = ng == 2 && static_cast<unsigned>(e1) < static_cast<unsigned>(p.n_blocks);
             vbits = (vbits & ~(3u << (2 * stage))) | ((v0 ? 1u : 0u) | (v1 ? 2u : 0u)) << (2 * stage);
             uint64_t* bar = &bars[warp][stage];
             uint8_t* dst = ring + stage * C::STAGE_BYTES;
             if (lane == 0) mbar_arrive_expect_tx(bar, ((v0 ? 1u : 0u) + (v1 ? 1u : 0u)) * C::GROUP);
-            __syncwarp();
-            const int h = pre.hr / p.n_rg;
-            if (p.bs_log2 == 4) {                                        // a group is a page: two copies
-                if (lane == 0 ? v0 : lane == 1 && v1)
-                    bulk_g2s(dst + lane * C::GROUP,
-                             p.cache + (static_cast<size_t>(lane ? e1 : e0) * p.H_kv + h) * page_bytes, C::GROUP, bar);
-            } else if (lane == 0 && v0) {                                // both groups lie in one page
-                const int gr = (key0 & ((1 << p.bs_log2) - 1)) >> 4;
-                bulk_g2s(dst, p.cache + (static_cast<size_t>(e0) * p.H_kv + h) * page_bytes + static_cast<size_t>(gr) * C::GROUP,
-                         ng * C::GROUP, bar);
+            const bool second = paired && lane == 1;
+            if (lane == 0 ? v0 : second && v1) {
+                const int e = second ? e1 : e0;
+                const uint32_t off = paired ? 0u : ((key0 & ((1u << p.bs_log2) - 1)) >> 4) * C::GROUP;
+                bulk_g2s(dst + (second ? C::GROUP : 0),
+                         p.cache + static_cast<uint64_t>(static_cast<uint32_t>(e * p.H_kv + pre.h)) * page_bytes + off,
+                         paired ? C::GROUP : ng * C::GROUP, bar);
             }
-            q4_advance(p, pre, HR);
+            q4_advance(p, pre);
+            // The next unit's queries on their way to L2 (a load behind the copies in flight waits for them).
+            if (pre.tile == 0 && pre.b < p.B) {
+                const char* q = reinterpret_cast<const char*>(
+                    p.Q + ((static_cast<size_t>(pre.b) * p.H_kv + pre.h) * p.R + pre.rg * C::ROWS) * D);
+                const int bytes = (p.R - pre.rg * C::ROWS < C::ROWS ? p.R - pre.rg * C::ROWS : C::ROWS) * D * 2;
+                for (int at = lane * 128; at < bytes; at += 32 * 128)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(q + at));
+            }
         };
 
+        uint4 raw[NT][C::KW];
+        q4_load_q<D, NT>(p, raw, cur, lane);                             // ahead of the copies
         int issued = y0;
         for (int i = 0; i < STAGES && issued < y1; ++i, ++issued) copy(i);
         Q4Warp<D, NT> s;
@@ -569,7 +621,8 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         int first = 0;
         for (int y = y0; y < y1; ++y) {
             if (fresh) {
-                q4_begin<D, NT>(p, s, cur, lane);
+                if (y != y0) q4_load_q<D, NT>(p, raw, cur, lane);
+                q4_begin<D, NT>(p, s, raw, cur, lane);
                 first = cur.tile;
                 fresh = false;
             }
@@ -578,8 +631,11 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                 if (ok) {
                     const uint32_t valid = (vbits >> (2 * stage)) & 3u;
                     const int key0 = cur.tile * 32;
-                    const bool masked = valid != 3u || key0 + 32 > cur.len - (p.causal ? p.S_q - 1 : 0);
-                    q4_tile<D, NT>(p, s, ring + stage * C::STAGE_BYTES, key0, cur.len, valid, masked, lane);
+                    const uint8_t* st = ring + stage * C::STAGE_BYTES;
+                    if (valid != 3u || key0 + 32 > cur.len - (p.causal ? p.S_q - 1 : 0))
+                        q4_tile<D, NT, true>(s, st, key0, cur.len, valid, lane);
+                    else
+                        q4_tile<D, NT, false>(s, st, key0, cur.len, valid, lane);
                     __syncwarp();
                     if (issued < y1) {
                         copy(stage);
@@ -604,23 +660,39 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
             const bool unit_end = cur.tile == cur.nt - 1, last = y == y1 - 1;
             if (unit_end || last) {
                 const bool whole = unit_end && first == 0;
-                const int u = cur.b * HR + cur.hr;
                 // A part that ends inside the warp's share goes to the warp's head slot, the last one to its ring.
                 float* part = last ? reinterpret_cast<float*>(ring) : heads + warp * C::PART_FLOATS;
                 __syncwarp();
-                q4_emit<D, NT>(p, s, u, whole, part, lane);
-                if (!whole && lane == 0) s_ent[2 * warp + (last ? 1 : 0)] = Q4Unit{u, y - cur.tile, cur.nt};
+                q4_emit<D, NT>(p, s, cur, whole, part, lane);
+                if (!whole && lane == 0)
+                    s_ent[2 * warp + (last ? 1 : 0)] = Q4Unit{q4_unit(p, cur), y - cur.tile, cur.nt};
                 fresh = true;
             }
-            q4_advance(p, cur, HR);
+            q4_advance(p, cur);
         }
     }
     __syncthreads();
 
     // ---- merge the CTA's parts: runs of equal units in the entries' order
-    const int n4 = NT * C::SETS * 4 * C::V4;
-    Q4Unit mine_u = lane < 2 * W ? s_ent[lane] : Q4Unit{-1, 0, 0};
+    constexpr int n4 = NT * C::SETS * 4 * C::V4;
+    auto entry = [&](int i) {
+        return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * STAGES * C::STAGE_BYTES)
+                     : heads + (i >> 1) * C::PART_FLOATS;
+    };
+    const Q4Unit mine_u = lane < 2 * W ? s_ent[lane] : Q4Unit{-1, 0, 0};
     uint32_t todo = __ballot_sync(0xffffffffu, mine_u.u >= 0);
+    // Each entry's weight per column.
+    for (int i = tid; i < 2 * W * C::ROWS; i += C::THREADS) {
+        const int e = i / C::ROWS, col = i % C::ROWS, u = s_ent[e].u;
+        if (u < 0) continue;
+        float M = -INFINITY;
+#pragma unroll
+        for (int f = 0; f < 2 * W; ++f)
+            if (s_ent[f].u == u) M = fmaxf(M, entry(f)[C::O_FLOATS + col]);
+        s_wt[e][col] = q4_weight(entry(e)[C::O_FLOATS + col], M);
+        s_mx[e][col] = M;
+    }
+    __syncthreads();
     int cross_u[2] = {-1, -1}, cross_first[2] = {0, 0}, cross_n[2] = {0, 0};
     while (todo) {
         const int lead = __ffs(todo) - 1;
@@ -633,25 +705,23 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         float* out = p.parts + (static_cast<size_t>(blockIdx.x) * 2 + slot) * C::PART_FLOATS;
         const int row0 = (u % p.n_rg) * C::ROWS;
         const size_t rbase = static_cast<size_t>(u / p.n_rg) * p.R;
+#pragma unroll 1
         for (int idx = tid; idx < n4 * 32; idx += C::THREADS) {
             const int ln = idx & 31, q4 = idx >> 5, v = q4 % C::V4, item = q4 / C::V4;
             const int e = item & 3, set = (item >> 2) % C::SETS, n = item / (4 * C::SETS);
             const int col = 8 * n + 2 * (ln & 3) + (e & 1), r = row0 + col;
-            auto entry = [&](int i) {
-                return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * STAGES * C::STAGE_BYTES)
-                             : heads + (i >> 1) * C::PART_FLOATS;
-            };
-            float M = -INFINITY, L = 0.f;
-            for (uint32_t b = run; b; b &= b - 1) M = fmaxf(M, entry(__ffs(b) - 1)[C::O_FLOATS + col]);
+            float L = 0.f;
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
             for (uint32_t b = run; b; b &= b - 1) {
-                const float* part = entry(__ffs(b) - 1);
-                const float w = q4_weight(part[C::O_FLOATS + col], M);
+                const int f = __ffs(b) - 1;
+                const float* part = entry(f);
+                const float w = s_wt[f][col];
                 const float4 y = reinterpret_cast<const float4*>(part)[q4 * 32 + ln];
                 L = fmaf(w, part[C::O_FLOATS + C::ROWS + col], L);
                 a.x = fmaf(w, y.x, a.x); a.y = fmaf(w, y.y, a.y); a.z = fmaf(w, y.z, a.z); a.w = fmaf(w, y.w, a.w);
             }
             const bool stats = (ln >> 2) == 0 && set == 0 && v == 0 && (e >> 1) == 0;
+            const float M = s_mx[lead][col];
             if (inside) {
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 if (r < p.R) {
@@ -669,12 +739,18 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
             }
         }
         if (!inside) {
-            // CTA of tile x: the largest c with floor(c T / act) <= x.
-            const int cf = static_cast<int>(((us + 1ll) * act - 1) / T);
-            const int cl = static_cast<int>((static_cast<long long>(us + unt) * act - 1) / T);
-            cross_u[slot] = u;
-            cross_first[slot] = cf;
-            cross_n[slot] = cl - cf + 1;
+            auto cta_of = [&](unsigned x) {
+                const unsigned big = rem * (quot + 1);
+                return static_cast<int>(x < big ? x / (quot + 1) : rem + (x - big) / quot);
+            };
+            const int cf = slot ? static_cast<int>(blockIdx.x) : cta_of(us), cl = cta_of(us + unt - 1);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (k == slot) {
+                    cross_u[k] = u;
+                    cross_first[k] = cf;
+                    cross_n[k] = cl - cf + 1;
+                }
         }
     }
     if (cross_u[0] < 0 && cross_u[1] < 0) return;
@@ -683,6 +759,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     __threadfence();
     __syncthreads();
     if (tid == 0) {
+#pragma unroll
         for (int k = 0; k < 2; ++k) {
             s_last[k] = 0;
             if (cross_u[k] >= 0 &&
@@ -694,9 +771,10 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     }
     __syncthreads();
     float* wm = reinterpret_cast<float*>(smem);                          // [parts][ROWS] m, then weights; [parts][ROWS] l; totals
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
         if (!s_last[k]) continue;
-        const int nparts = cross_n[k], cf = cross_first[k], u = cross_u[k];
+        const int nparts = k ? cross_n[1] : cross_n[0], cf = k ? cross_first[1] : cross_first[0], u = k ? cross_u[1] : cross_u[0];
         float* wl = wm + nparts * C::ROWS;
         float* tot = wl + nparts * C::ROWS;                              // M, L per column
         auto part = [&](int i) { return p.parts + (static_cast<size_t>(cf + i) * 2 + (i == 0 ? 1 : 0)) * C::PART_FLOATS; };
