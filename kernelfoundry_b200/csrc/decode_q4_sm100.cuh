@@ -77,7 +77,7 @@ struct Q4AttnCfg {
     static constexpr int PART_FLOATS = O_FLOATS + 2 * ROWS;      // O, m, l
     static constexpr int RING_BYTES = W * STAGES * STAGE_BYTES;
     static constexpr int SMEM_BYTES = RING_BYTES + W * PART_FLOATS * 4;
-    static_assert(STAGES * STAGE_BYTES >= PART_FLOATS * 4, "a warp's last part is kept in its ring");
+    static_assert(STAGES <= 16 && STAGES * STAGE_BYTES >= PART_FLOATS * 4, "a warp's last part is kept in its ring");
     static_assert(SMEM_BYTES <= 225 * 1024, "shared memory");
 };
 
@@ -145,8 +145,7 @@ __device__ __forceinline__ int q4_len(const Q4AttnParams& p, int b) {
 // Tiles of a sequence: an empty one keeps one (masked) tile, whose unit writes the zeros.
 __device__ __forceinline__ int q4_tiles(int len) { return len <= 32 ? 1 : (len + 31) >> 5; }
 
-__device__ __forceinline__ void q4_advance(const Q4AttnParams& p, Q4Cursor& c) {
-    if (++c.tile < c.nt) return;
+__device__ __forceinline__ void q4_next_unit(const Q4AttnParams& p, Q4Cursor& c) {
     c.tile = 0;
     if (++c.rg < p.n_rg) return;
     c.rg = 0;
@@ -477,6 +476,9 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
         }
 }
 
+// What the merge of a unit across CTAs costs, in tiles of one CTA.
+constexpr unsigned kQ4MergeTiles = 32;
+
 __device__ __forceinline__ float q4_weight(float m, float M) { return m == -INFINITY ? 0.f : ex2_approx(m - M); }
 
 template <int D, int NT>
@@ -489,6 +491,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     __shared__ int s_sum[W];
     __shared__ int s_b[W], s_base[W];
     __shared__ Q4Unit s_ent[2 * W];
+    __shared__ int s_list[2 * W];
     __shared__ float s_wt[2 * W][C::ROWS], s_mx[2 * W][C::ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* heads = reinterpret_cast<float*>(smem + C::RING_BYTES);
@@ -508,7 +511,13 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     const int per = (p.B + C::THREADS - 1) / C::THREADS;
     const int b0 = tid * per < p.B ? tid * per : p.B, b1 = b0 + per < p.B ? b0 + per : p.B;
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += q4_tiles(q4_len(p, b));
+    const int nt0 = q4_tiles(q4_len(p, 0));
+    bool same = true;
+    for (int b = b0; b < b1; ++b) {
+        const int nt = q4_tiles(q4_len(p, b));
+        mine += nt;
+        same = same && nt == nt0;
+    }
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -516,7 +525,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         if (lane >= o) incl += v;
     }
     if (lane == 31) s_sum[warp] = incl;
-    __syncthreads();
+    const bool s_same = __syncthreads_and(same);
     unsigned total = 0, before = incl - mine;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -527,10 +536,22 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     const unsigned T = total * HR;                                       // < 2^31, the host sees to it
     // CTAs that take part: every warp of theirs gets at least a tile.  CTA c has the tiles from
     // c * quot + min(c, rem), warp w of it those from x0 + w * (x1 - x0) / W.
-    const unsigned want = (T + W - 1) / W, act = want < gridDim.x ? want : gridDim.x;
+    const unsigned want = (T + W - 1) / W;
+    unsigned act = want < gridDim.x ? want : gridDim.x, quot = T / act, rem = T - quot * act;
+    // Sequences of one length: whole units to each CTA, if that takes no longer than an even
+    // split and the merge across CTAs that it needs.
+    if (s_same) {
+        const unsigned units = p.B * HR, nt = total / p.B, each = (units + gridDim.x - 1) / gridDim.x;
+        if (each * nt <= quot + kQ4MergeTiles) {
+            act = (units + each - 1) / each;
+            quot = each * nt;
+            rem = 0;
+        }
+    }
     if (blockIdx.x >= act) return;
-    const unsigned quot = T / act, rem = T - quot * act;
-    const int x0 = blockIdx.x * quot + (blockIdx.x < rem ? blockIdx.x : rem), x1 = x0 + quot + (blockIdx.x < rem ? 1 : 0);
+    const int x0 = blockIdx.x * quot + (blockIdx.x < rem ? blockIdx.x : rem);
+    int x1 = x0 + quot + (blockIdx.x < rem ? 1 : 0);
+    if (blockIdx.x == act - 1) x1 = T;
     const int wq = (x1 - x0) / W, wr = (x1 - x0) % W;
     auto warp_start = [&](int w) { return x0 + w * wq + (w < wr ? w : wr); };
     if (mine > 0) {
@@ -553,6 +574,8 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
 
     const int y0 = warp_start(warp), y1 = warp_start(warp + 1);
     if (y0 < y1) {
+        int y_cur = y0;                                                  // the tile in work
+        uint32_t vbits = 0;                                              // 2 validity bits per stage
         Q4Cursor cur;
         cur.b = s_b[warp];
         cur.len = q4_len(p, cur.b);
@@ -567,108 +590,127 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                 cur.rg = hr - cur.h * p.n_rg;
             }
         }
-        Q4Cursor pre = cur;                                              // next tile to copy
-        int win = -1, win_b = -1, win_p = 0;                             // 32 table entries, one per lane
-        uint32_t vbits = 0;                                              // 2 validity bits per stage
-        const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
-        const bool paired = p.bs_log2 == 4;                              // a group is a page: a tile takes two copies
+        uint4 raw[NT][C::KW];
+        q4_load_q<D, NT>(p, raw, cur, lane);                             // ahead of the copies
 
-        auto copy = [&](int stage) {
-            const int key0 = pre.tile * 32, rem = pre.len - key0;
-            const int ng = rem <= 0 ? 0 : rem <= 16 ? 1 : 2;
-            const int p0 = key0 >> p.bs_log2;
-            if (ng && (pre.b != win_b || static_cast<unsigned>(p0 - win_p) >= 31u)) {
-                win_b = pre.b;
-                win_p = p0;
-                const int used = (pre.len + (1 << p.bs_log2) - 1) >> p.bs_log2;
-                win = p0 + lane < used ? p.table[static_cast<size_t>(pre.b) * p.max_blocks + p0 + lane] : -1;
+        // Copies.  Lane i holds what tile win0 + i needs and issues its copy; the window is
+        // refilled every 32 tiles.
+        int issued = y0, win0 = y0;
+        const uint8_t* src0 = nullptr;
+        const uint8_t* src1 = nullptr;                                   // 16-token pages: the second group's
+        uint32_t bytes = 0, first_ok = 0, second_ok = 0;
+        const bool paired = p.bs_log2 == 4;
+        auto refill = [&]() {
+            win0 = issued;
+            int b = cur.b, len = cur.len, nt = cur.nt;
+            unsigned off = (cur.h * p.n_rg + cur.rg) * nt + cur.tile + (issued - y_cur) + lane;
+            const bool mine_t = issued + lane < y1;
+            while (mine_t && off >= static_cast<unsigned>(HR * nt)) {
+                off -= HR * nt;
+                len = q4_len(p, ++b);
+                nt = q4_tiles(len);
             }
-            const int e0 = __shfl_sync(0xffffffffu, win, p0 - win_p);
-            const int e1 = paired ? __shfl_sync(0xffffffffu, win, p0 - win_p + 1) : e0;
-            const bool v0 = ng >= 1 && static_cast<unsigned>(e0) < static_cast<unsigned>(p.n_blocks);
-            const bool v1 = ng == 2 && static_cast<unsigned>(e1) < static_cast<unsigned>(p.n_blocks);
-            vbits = (vbits & ~(3u << (2 * stage))) | ((v0 ? 1u : 0u) | (v1 ? 2u : 0u)) << (2 * stage);
-            uint64_t* bar = &bars[warp][stage];
-            uint8_t* dst = ring + stage * C::STAGE_BYTES;
-            if (lane == 0) mbar_arrive_expect_tx(bar, ((v0 ? 1u : 0u) + (v1 ? 1u : 0u)) * C::GROUP);
-            const bool second = paired && lane == 1;
-            if (lane == 0 ? v0 : second && v1) {
-                const int e = second ? e1 : e0;
-                const uint32_t off = paired ? 0u : ((key0 & ((1u << p.bs_log2) - 1)) >> 4) * C::GROUP;
-                bulk_g2s(dst + (second ? C::GROUP : 0),
-                         p.cache + static_cast<uint64_t>(static_cast<uint32_t>(e * p.H_kv + pre.h)) * page_bytes + off,
-                         paired ? C::GROUP : ng * C::GROUP, bar);
-            }
-            q4_advance(p, pre);
-            // The next unit's queries on their way to L2 (a load behind the copies in flight waits for them).
-            if (pre.tile == 0 && pre.b < p.B) {
-                const char* q = reinterpret_cast<const char*>(
-                    p.Q + ((static_cast<size_t>(pre.b) * p.H_kv + pre.h) * p.R + pre.rg * C::ROWS) * D);
-                const int bytes = (p.R - pre.rg * C::ROWS < C::ROWS ? p.R - pre.rg * C::ROWS : C::ROWS) * D * 2;
-                for (int at = lane * 128; at < bytes; at += 32 * 128)
+            const unsigned hr = off / nt, tile = off - hr * nt, h = p.n_rg == 1 ? hr : hr / p.n_rg;
+            const int left = len - static_cast<int>(tile) * 32;
+            const int ng = !mine_t || left <= 0 ? 0 : left <= 16 ? 1 : 2;
+            const unsigned page = (tile * 32) >> p.bs_log2;
+            const int* row = p.table + static_cast<size_t>(b) * p.max_blocks + page;
+            const unsigned e0 = ng >= 1 ? row[0] : 0xffffffffu;
+            const unsigned e1 = ng == 2 ? (paired ? row[1] : static_cast<int>(e0)) : 0xffffffffu;
+            const bool v0 = e0 < static_cast<unsigned>(p.n_blocks), v1 = e1 < static_cast<unsigned>(p.n_blocks);
+            const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
+            const uint32_t in_page = ((tile * 32) & ((1u << p.bs_log2) - 1)) >> 4;
+            src0 = p.cache + static_cast<uint64_t>(e0 * p.H_kv + h) * page_bytes + in_page * C::GROUP;
+            src1 = p.cache + static_cast<uint64_t>(e1 * p.H_kv + h) * page_bytes;
+            bytes = ((v0 ? 1u : 0u) + (v1 ? 1u : 0u)) * C::GROUP;
+            first_ok = __ballot_sync(0xffffffffu, v0);
+            second_ok = __ballot_sync(0xffffffffu, v1);
+            // A unit that begins in this window: its queries on their way to L2 (a load behind
+            // the copies in flight would wait for them).
+            if (mine_t && tile == 0 && issued + lane != y0) {
+                const unsigned rg = hr - h * p.n_rg, rows = p.R - rg * C::ROWS;
+                const char* q = reinterpret_cast<const char*>(p.Q + ((static_cast<size_t>(b) * p.H_kv + h) * p.R + rg * C::ROWS) * D);
+                for (unsigned at = 0; at < (rows < C::ROWS ? rows : C::ROWS) * D * 2; at += 128)
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(q + at));
             }
         };
+        auto issue = [&](int stage) {
+            if (lane == issued - win0) {
+                uint64_t* bar = &bars[warp][stage];
+                uint8_t* dst = ring + stage * C::STAGE_BYTES;
+                mbar_arrive_expect_tx(bar, bytes);
+                if (!paired) {
+                    if (bytes) bulk_g2s(dst, src0, bytes, bar);          // both groups lie in one page
+                } else {
+                    if ((first_ok >> lane) & 1u) bulk_g2s(dst, src0, C::GROUP, bar);
+                    if ((second_ok >> lane) & 1u) bulk_g2s(dst + C::GROUP, src1, C::GROUP, bar);
+                }
+            }
+            const uint32_t v = ((first_ok >> (issued - win0)) & 1u) | (((second_ok >> (issued - win0)) & 1u) << 1);
+            vbits = (vbits & ~(3u << (2 * stage))) | v << (2 * stage);
+            ++issued;
+        };
 
-        uint4 raw[NT][C::KW];
-        q4_load_q<D, NT>(p, raw, cur, lane);                             // ahead of the copies
-        int issued = y0;
-        for (int i = 0; i < STAGES && issued < y1; ++i, ++issued) copy(i);
+        refill();
+#pragma unroll 1
+        for (int i = 0; i < STAGES && issued < y1; ++i) issue(i);
         Q4Warp<D, NT> s;
         int stage = 0;
         uint32_t phase = 0;
-        bool ok = true, fresh = true;
-        int first = 0;
-        for (int y = y0; y < y1; ++y) {
-            if (fresh) {
-                if (y != y0) q4_load_q<D, NT>(p, raw, cur, lane);
-                q4_begin<D, NT>(p, s, raw, cur, lane);
-                first = cur.tile;
-                fresh = false;
-            }
-            if (ok) {
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars[warp][stage], phase, &s_abort, p.timeout_ns));
-                if (ok) {
-                    const uint32_t valid = (vbits >> (2 * stage)) & 3u;
-                    const int key0 = cur.tile * 32;
-                    const uint8_t* st = ring + stage * C::STAGE_BYTES;
-                    if (valid != 3u || key0 + 32 > cur.len - (p.causal ? p.S_q - 1 : 0))
-                        q4_tile<D, NT, true>(s, st, key0, cur.len, valid, lane);
-                    else
-                        q4_tile<D, NT, false>(s, st, key0, cur.len, valid, lane);
-                    __syncwarp();
-                    if (issued < y1) {
-                        copy(stage);
-                        ++issued;
-                    }
-                } else {
+        bool ok = true;
+#pragma unroll 1
+        while (y_cur < y1) {                                             // a unit, or the warp's share of it
+            q4_begin<D, NT>(p, s, raw, cur, lane);
+            const int first = cur.tile, n = cur.nt - first < y1 - y_cur ? cur.nt - first : y1 - y_cur;
+            const int plain_end = cur.len - (p.causal ? p.S_q - 1 : 0) - 32;   // key0 up to here: all rows see all keys
+#pragma unroll 1
+            for (int i = 0; i < n && ok; ++i) {
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[warp][stage], phase, &s_abort, p.timeout_ns))) {
                     // The copies in flight still land in this ring: wait for them (bounded) before leaving it.
                     if (lane == 0) atomicOr(&g_kf_dev_error, KF_DEVERR_TIMEOUT_TMA);
-                    for (int z = y, sz = stage, pz = phase; z < issued; ++z) {
+                    for (int z = y_cur, sz = stage, pz = phase; z < issued; ++z) {
                         s_drop[warp] = 0;
                         __syncwarp();
                         mbar_wait_bounded(&bars[warp][sz], pz, &s_drop[warp], p.timeout_ns);
                         __syncwarp();
                         if (++sz == STAGES) { sz = 0; pz ^= 1; }
                     }
+                    ok = false;
+                    break;
+                }
+                const uint32_t valid = (vbits >> (2 * stage)) & 3u;
+                const int key0 = cur.tile * 32;
+                const uint8_t* st = ring + stage * C::STAGE_BYTES;
+                if (valid != 3u || key0 > plain_end) q4_tile<D, NT, true>(s, st, key0, cur.len, valid, lane);
+                else q4_tile<D, NT, false>(s, st, key0, cur.len, valid, lane);
+                ++cur.tile;
+                ++y_cur;
+                __syncwarp();
+                if (issued < y1) {
+                    if (issued - win0 == 32) refill();
+                    issue(stage);
                 }
                 if (++stage == STAGES) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
-            const bool unit_end = cur.tile == cur.nt - 1, last = y == y1 - 1;
-            if (unit_end || last) {
-                const bool whole = unit_end && first == 0;
-                // A part that ends inside the warp's share goes to the warp's head slot, the last one to its ring.
-                float* part = last ? reinterpret_cast<float*>(ring) : heads + warp * C::PART_FLOATS;
-                __syncwarp();
-                q4_emit<D, NT>(p, s, cur, whole, part, lane);
-                if (!whole && lane == 0)
-                    s_ent[2 * warp + (last ? 1 : 0)] = Q4Unit{q4_unit(p, cur), y - cur.tile, cur.nt};
-                fresh = true;
+            if (!ok) {                                                   // (the parts still go through the merge)
+                y_cur += first + n - cur.tile;
+                cur.tile = first + n;
             }
-            q4_advance(p, cur);
+            const bool whole = n == cur.nt, last = y_cur >= y1;
+            // A part that ends inside the warp's share goes to the warp's head slot, the last one to its ring.
+            float* part = last ? reinterpret_cast<float*>(ring) : heads + warp * C::PART_FLOATS;
+            __syncwarp();
+            const Q4Cursor done = cur;
+            if (!last) {
+                q4_next_unit(p, cur);
+                q4_load_q<D, NT>(p, raw, cur, lane);
+            }
+            q4_emit<D, NT>(p, s, done, whole, part, lane);
+            if (!whole && lane == 0)
+                s_ent[2 * warp + (last ? 1 : 0)] = Q4Unit{q4_unit(p, done), y_cur - done.tile, done.nt};
         }
     }
     __syncthreads();
@@ -680,25 +722,34 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                      : heads + (i >> 1) * C::PART_FLOATS;
     };
     const Q4Unit mine_u = lane < 2 * W ? s_ent[lane] : Q4Unit{-1, 0, 0};
-    uint32_t todo = __ballot_sync(0xffffffffu, mine_u.u >= 0);
-    // Each entry's weight per column.
-    for (int i = tid; i < 2 * W * C::ROWS; i += C::THREADS) {
-        const int e = i / C::ROWS, col = i % C::ROWS, u = s_ent[e].u;
-        if (u < 0) continue;
-        float M = -INFINITY;
+    const uint32_t used = __ballot_sync(0xffffffffu, mine_u.u >= 0);
+    if (warp == 0 && mine_u.u >= 0) s_list[__popc(used & ((1u << lane) - 1))] = lane;
+    // Each entry's weight per column, a lane an entry.
+    for (int col = warp; col < C::ROWS; col += W) {
+        const float m = mine_u.u >= 0 ? entry(lane)[C::O_FLOATS + col] : -INFINITY;
+        for (uint32_t todo = used; todo;) {
+            const uint32_t run = __ballot_sync(0xffffffffu, mine_u.u == __shfl_sync(0xffffffffu, mine_u.u, __ffs(todo) - 1));
+            todo &= ~run;
+            const bool in = (run >> lane) & 1u;
+            float M = in ? m : -INFINITY;
 #pragma unroll
-        for (int f = 0; f < 2 * W; ++f)
-            if (s_ent[f].u == u) M = fmaxf(M, entry(f)[C::O_FLOATS + col]);
-        s_wt[e][col] = q4_weight(entry(e)[C::O_FLOATS + col], M);
-        s_mx[e][col] = M;
+            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+            if (in) {
+                s_wt[lane][col] = q4_weight(m, M);
+                s_mx[lane][col] = M;
+            }
+        }
     }
     __syncthreads();
     int cross_u[2] = {-1, -1}, cross_first[2] = {0, 0}, cross_n[2] = {0, 0};
-    while (todo) {
+    int at = 0;
+    for (uint32_t todo = used; todo;) {
         const int lead = __ffs(todo) - 1;
         const int u = __shfl_sync(0xffffffffu, mine_u.u, lead);
         const int us = __shfl_sync(0xffffffffu, mine_u.start, lead), unt = __shfl_sync(0xffffffffu, mine_u.nt, lead);
         const uint32_t run = __ballot_sync(0xffffffffu, mine_u.u == u);
+        const int from = at, to = at + __popc(run);
+        at = to;
         todo &= ~run;
         const bool inside = us >= x0 && us + unt <= x1;
         const int slot = us >= x0 ? 1 : 0;
@@ -712,8 +763,9 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
             const int col = 8 * n + 2 * (ln & 3) + (e & 1), r = row0 + col;
             float L = 0.f;
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t b = run; b; b &= b - 1) {
-                const int f = __ffs(b) - 1;
+#pragma unroll 4
+            for (int i = from; i < to; ++i) {
+                const int f = s_list[i];
                 const float* part = entry(f);
                 const float w = s_wt[f][col];
                 const float4 y = reinterpret_cast<const float4*>(part)[q4 * 32 + ln];
@@ -756,9 +808,8 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     if (cross_u[0] < 0 && cross_u[1] < 0) return;
 
     // ---- units that cross CTAs: the last CTA to arrive merges the parts, in CTA order
-    __threadfence();
     __syncthreads();
-    if (tid == 0) {
+    if (tid == 0) {                                                      // (its release covers what the barrier ordered before)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             s_last[k] = 0;
