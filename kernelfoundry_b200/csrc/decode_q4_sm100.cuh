@@ -124,6 +124,7 @@ struct Q4Warp {                    // a warp's running state of one unit; pairs:
     uint32_t q[NT][Q4AttnCfg<D, NT>::KW][4];
     float2 cq[NT];                 // a column's factor of the scores
     int lim[NT][2];                // keys the column's query sees
+    float tmx;                     // this thread's largest value scale
     float tlim, tnorm, tinv;       // value scales up to tlim times tnorm stay below 2^7; tinv = 1 / tnorm
 };
 
@@ -184,7 +185,7 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
                                          const Q4Cursor& c, int lane) {
     using C = Q4AttnCfg<D, NT>;
     const int t = lane & 3;
-    s.tlim = 0.f;
+    s.tmx = s.tlim = 0.f;
     s.tnorm = s.tinv = 1.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -294,17 +295,17 @@ __device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int
         }
     }
     // Does a score pass m + 8, or a value scale the range of p t?  Rarely.
-    float2 mx[NT];
-    const float tm = fmaxf(fmaxf(tv[0][0], tv[0][1]), fmaxf(tv[1][0], tv[1][1]));   // (a spoiled row's NaN is ignored)
-    bool up = tm > s.tlim;
+    s.tmx = fmax3f(s.tmx, tv[0][0], tv[0][1]);                               // (a spoiled row's NaN is ignored)
+    s.tmx = fmax3f(s.tmx, tv[1][0], tv[1][1]);
+    bool up = s.tmx > s.tlim;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        mx[n] = fmax2(fmax2(x[0][n][0], x[0][n][1]), fmax2(x[1][n][0], x[1][n][1]));
-        s.mt[n] = fmax2(s.mt[n], mx[n]);
-        up = up || mx[n].x > s.m[n].x + 8.0f || mx[n].y > s.m[n].y + 8.0f;
+        s.mt[n].x = fmax3f(fmax3f(s.mt[n].x, x[0][n][0].x, x[0][n][1].x), x[1][n][0].x, x[1][n][1].x);
+        s.mt[n].y = fmax3f(fmax3f(s.mt[n].y, x[0][n][0].y, x[0][n][1].y), x[1][n][0].y, x[1][n][1].y);
+        up = up || s.mt[n].x > s.m[n].x + 8.0f || s.mt[n].y > s.m[n].y + 8.0f;
     }
     if (__any_sync(0xffffffffu, up)) {
-        const float tt = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(tm, 0.f))));
+        const float tt = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s.tmx)));
         float r = 1.0f;
         if (tt > s.tlim) {
             int e = static_cast<int>(__float_as_uint(tt) >> 23);             // 27 or more: scales are 0 or >= 2^-100
@@ -316,14 +317,13 @@ __device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float v[2] = {mx[n].x, mx[n].y}, a[2];
+            float v[2] = {s.mt[n].x, s.mt[n].y}, a[2];
             float m[2] = {s.m[n].x, s.m[n].y}, ms[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 4));
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 8));
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 16));
-                v[k] = fmaxf(v[k], m[k]);
                 ms[k] = v[k] == -INFINITY ? 0.f : v[k];
                 a[k] = ex2_approx(m[k] - ms[k]);
             }
@@ -488,6 +488,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[W][STAGES];
     __shared__ int s_abort, s_drop[W], s_last[2];
+    __shared__ uint32_t s_valid[W][STAGES];                              // groups copied, 2 bits
     __shared__ int s_sum[W];
     __shared__ int s_b[W], s_base[W];
     __shared__ Q4Unit s_ent[2 * W];
@@ -575,7 +576,6 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     const int y0 = warp_start(warp), y1 = warp_start(warp + 1);
     if (y0 < y1) {
         int y_cur = y0;                                                  // the tile in work
-        uint32_t vbits = 0;                                              // 2 validity bits per stage
         Q4Cursor cur;
         cur.b = s_b[warp];
         cur.len = q4_len(p, cur.b);
@@ -593,65 +593,70 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         uint4 raw[NT][C::KW];
         q4_load_q<D, NT>(p, raw, cur, lane);                             // ahead of the copies
 
-        // Copies.  Lane i holds what tile win0 + i needs and issues its copy; the window is
-        // refilled every 32 tiles.
+        // Copies.  Lane i holds what tile win0 + i needs and issues its copy.  The window moves on
+        // every 32 tiles; the table entries of the next one are loaded when it does (a load waits
+        // behind the copies in flight for microseconds).
         int issued = y0, win0 = y0;
         const uint8_t* src0 = nullptr;
         const uint8_t* src1 = nullptr;                                   // 16-token pages: the second group's
-        uint32_t bytes = 0, first_ok = 0, second_ok = 0;
+        uint32_t bytes = 0, valid = 0;
         const bool paired = p.bs_log2 == 4;
-        auto refill = [&]() {
-            win0 = issued;
-            int b = cur.b, len = cur.len, nt = cur.nt;
-            unsigned off = (cur.h * p.n_rg + cur.rg) * nt + cur.tile + (issued - y_cur) + lane;
-            const bool mine_t = issued + lane < y1;
-            while (mine_t && off >= static_cast<unsigned>(HR * nt)) {
-                off -= HR * nt;
-                len = q4_len(p, ++b);
-                nt = q4_tiles(len);
+        unsigned e0 = 0, e1 = 0, e_at = 0;                               // entries to come, (head << 4 | group in the page), groups
+        auto fetch = [&](int y) {                                        // for the window that begins at tile y
+            e0 = e1 = 0xffffffffu;
+            if (y + lane < y1) {
+                int b = cur.b, len = cur.len, nt = cur.nt;
+                unsigned off = (cur.h * p.n_rg + cur.rg) * nt + cur.tile + (y - y_cur) + lane;
+                while (off >= static_cast<unsigned>(HR * nt)) {
+                    off -= HR * nt;
+                    len = q4_len(p, ++b);
+                    nt = q4_tiles(len);
+                }
+                const unsigned hr = off / nt, tile = off - hr * nt, h = p.n_rg == 1 ? hr : hr / p.n_rg;
+                const int left = len - static_cast<int>(tile) * 32;
+                const unsigned page = (tile * 32) >> p.bs_log2;
+                const int* row = p.table + static_cast<size_t>(b) * p.max_blocks + page;
+                e_at = h << 4 | ((tile * 32) & ((1u << p.bs_log2) - 1)) >> 4;
+                if (left > 0) e0 = row[0];
+                if (left > 16) e1 = row[paired ? 1 : 0];
+                // A unit that begins here: its queries on their way to L2, for the same reason.
+                if (tile == 0 && y + lane != y0) {
+                    const unsigned rg = hr - h * p.n_rg, rows = p.R - rg * C::ROWS;
+                    const char* q = reinterpret_cast<const char*>(
+                        p.Q + ((static_cast<size_t>(b) * p.H_kv + h) * p.R + rg * C::ROWS) * D);
+                    for (unsigned at = 0; at < (rows < C::ROWS ? rows : C::ROWS) * D * 2; at += 128)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(q + at));
+                }
             }
-            const unsigned hr = off / nt, tile = off - hr * nt, h = p.n_rg == 1 ? hr : hr / p.n_rg;
-            const int left = len - static_cast<int>(tile) * 32;
-            const int ng = !mine_t || left <= 0 ? 0 : left <= 16 ? 1 : 2;
-            const unsigned page = (tile * 32) >> p.bs_log2;
-            const int* row = p.table + static_cast<size_t>(b) * p.max_blocks + page;
-            const unsigned e0 = ng >= 1 ? row[0] : 0xffffffffu;
-            const unsigned e1 = ng == 2 ? (paired ? row[1] : static_cast<int>(e0)) : 0xffffffffu;
+        };
+        auto move_on = [&]() {
+            win0 = issued;
             const bool v0 = e0 < static_cast<unsigned>(p.n_blocks), v1 = e1 < static_cast<unsigned>(p.n_blocks);
             const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
-            const uint32_t in_page = ((tile * 32) & ((1u << p.bs_log2) - 1)) >> 4;
-            src0 = p.cache + static_cast<uint64_t>(e0 * p.H_kv + h) * page_bytes + in_page * C::GROUP;
-            src1 = p.cache + static_cast<uint64_t>(e1 * p.H_kv + h) * page_bytes;
+            src0 = p.cache + static_cast<uint64_t>(e0 * p.H_kv + (e_at >> 4)) * page_bytes + (e_at & 15u) * C::GROUP;
+            src1 = p.cache + static_cast<uint64_t>(e1 * p.H_kv + (e_at >> 4)) * page_bytes;
             bytes = ((v0 ? 1u : 0u) + (v1 ? 1u : 0u)) * C::GROUP;
-            first_ok = __ballot_sync(0xffffffffu, v0);
-            second_ok = __ballot_sync(0xffffffffu, v1);
-            // A unit that begins in this window: its queries on their way to L2 (a load behind
-            // the copies in flight would wait for them).
-            if (mine_t && tile == 0 && issued + lane != y0) {
-                const unsigned rg = hr - h * p.n_rg, rows = p.R - rg * C::ROWS;
-                const char* q = reinterpret_cast<const char*>(p.Q + ((static_cast<size_t>(b) * p.H_kv + h) * p.R + rg * C::ROWS) * D);
-                for (unsigned at = 0; at < (rows < C::ROWS ? rows : C::ROWS) * D * 2; at += 128)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(q + at));
-            }
+            valid = (v0 ? 1u : 0u) | (v1 ? 2u : 0u);
+            if (win0 + 32 < y1) fetch(win0 + 32);
         };
         auto issue = [&](int stage) {
             if (lane == issued - win0) {
                 uint64_t* bar = &bars[warp][stage];
                 uint8_t* dst = ring + stage * C::STAGE_BYTES;
+                s_valid[warp][stage] = valid;
                 mbar_arrive_expect_tx(bar, bytes);
                 if (!paired) {
                     if (bytes) bulk_g2s(dst, src0, bytes, bar);          // both groups lie in one page
                 } else {
-                    if ((first_ok >> lane) & 1u) bulk_g2s(dst, src0, C::GROUP, bar);
-                    if ((second_ok >> lane) & 1u) bulk_g2s(dst + C::GROUP, src1, C::GROUP, bar);
+                    if (valid & 1u) bulk_g2s(dst, src0, C::GROUP, bar);
+                    if (valid & 2u) bulk_g2s(dst + C::GROUP, src1, C::GROUP, bar);
                 }
             }
-            const uint32_t v = ((first_ok >> (issued - win0)) & 1u) | (((second_ok >> (issued - win0)) & 1u) << 1);
-            vbits = (vbits & ~(3u << (2 * stage))) | v << (2 * stage);
             ++issued;
         };
 
-        refill();
+        fetch(y0);
+        move_on();
 #pragma unroll 1
         for (int i = 0; i < STAGES && issued < y1; ++i) issue(i);
         Q4Warp<D, NT> s;
@@ -678,16 +683,16 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                     ok = false;
                     break;
                 }
-                const uint32_t valid = (vbits >> (2 * stage)) & 3u;
+                const uint32_t got = s_valid[warp][stage];
                 const int key0 = cur.tile * 32;
                 const uint8_t* st = ring + stage * C::STAGE_BYTES;
-                if (valid != 3u || key0 > plain_end) q4_tile<D, NT, true>(s, st, key0, cur.len, valid, lane);
-                else q4_tile<D, NT, false>(s, st, key0, cur.len, valid, lane);
+                if (got != 3u || key0 > plain_end) q4_tile<D, NT, true>(s, st, key0, cur.len, got, lane);
+                else q4_tile<D, NT, false>(s, st, key0, cur.len, got, lane);
                 ++cur.tile;
                 ++y_cur;
                 __syncwarp();
                 if (issued < y1) {
-                    if (issued - win0 == 32) refill();
+                    if (issued - win0 == 32) move_on();
                     issue(stage);
                 }
                 if (++stage == STAGES) {
