@@ -434,52 +434,141 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
     const int row0 = c.rg * C::ROWS;
     const size_t rbase = (static_cast<size_t>(c.b) * p.H_kv + c.h) * p.R;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+        float2 l = s.l[n], m = s.mt[n];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            float l = k ? s.l[n].y : s.l[n].x, m = k ? s.mt[n].y : s.mt[n].x;
+        for (int o = 4; o < 32; o <<= 1) {
+            l = fadd2(l, make_float2(__shfl_xor_sync(0xffffffffu, l.x, o), __shfl_xor_sync(0xffffffffu, l.y, o)));
+            m = fmax2(m, make_float2(__shfl_xor_sync(0xffffffffu, m.x, o), __shfl_xor_sync(0xffffffffu, m.y, o)));
+        }
+        // From the exponent's reference to the true maximum (at most 8 above it).
+        const float2 a = make_float2(m.x == -INFINITY ? 1.0f : ex2_approx(s.m[n].x - m.x),
+                                     m.y == -INFINITY ? 1.0f : ex2_approx(s.m[n].y - m.y));
+        l = fmul2(l, a);
+        float2 f = fmul2(a, make_float2(s.tinv, s.tinv));
+        if (whole) f = fmul2(f, make_float2(l.x == 0.f ? 0.f : 1.0f / l.x, l.y == 0.f ? 0.f : 1.0f / l.y));
+        const int col = 8 * n + 2 * t;
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                l += __shfl_xor_sync(0xffffffffu, l, o);
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            }
-            // From the exponent's reference to the true maximum (at most 8 above it).
-            const float a = m == -INFINITY ? 1.0f : ex2_approx((k ? s.m[n].y : s.m[n].x) - m);
-            l *= a;
-            const int col = 8 * n + 2 * t + k, r = row0 + col;
-            const float f = whole ? s.tinv * a * (l == 0.f ? 0.f : 1.0f / l) : s.tinv * a;
+        for (int set = 0; set < C::SETS; ++set)
 #pragma unroll
-            for (int set = 0; set < C::SETS; ++set)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int v = 0; v < C::V4; ++v) {
+                    float2 y[4];                                             // 2^9 by itself: with f it could leave fp32's range
 #pragma unroll
-                    for (int v = 0; v < C::V4; ++v) {
-                        float y[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) y[i] = s.o[n][set * 8 + 4 * v + i][2 * h + k] * 0x1p9f * f;
-                        const float4 y4 = make_float4(y[0], y[1], y[2], y[3]);
-                        const int e = 2 * h + k;
-                        if (!whole)
-                            reinterpret_cast<float4*>(part)[(((n * C::SETS + set) * 4 + e) * C::V4 + v) * 32 + lane] = y4;
-                        else if (r < p.R)
-                            store_out4(p.O, (rbase + r) * D + q4_dim<D>(set, e, v, g), y4, p.out_type);
+                    for (int i = 0; i < 4; ++i) {
+                        const float(&o)[4] = s.o[n][set * 8 + 4 * v + i];
+                        y[i] = fmul2(fmul2(make_float2(o[2 * h], o[2 * h + 1]), make_float2(0x1p9f, 0x1p9f)), f);
                     }
-            if (g == 0) {
+                    const float4 y0 = make_float4(y[0].x, y[1].x, y[2].x, y[3].x), y1 = make_float4(y[0].y, y[1].y, y[2].y, y[3].y);
+                    if (!whole) {
+                        float4* at = reinterpret_cast<float4*>(part) + (((n * C::SETS + set) * 4 + 2 * h) * C::V4 + v) * 32 + lane;
+                        at[0] = y0;
+                        at[C::V4 * 32] = y1;
+                    } else {
+                        const size_t at = (rbase + row0 + col) * D + q4_dim<D>(set, 2 * h, v, g);
+                        if (row0 + col < p.R) store_out4(p.O, at, y0, p.out_type);
+                        if (row0 + col + 1 < p.R) store_out4(p.O, at + D, y1, p.out_type);
+                    }
+                }
+        if (g == 0) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float mk = k ? m.y : m.x, lk = k ? l.y : l.x;
                 if (!whole) {
-                    part[C::O_FLOATS + col] = m;
-                    part[C::O_FLOATS + C::ROWS + col] = l;
-                } else if (r < p.R) {
-                    if (p.Mi) p.Mi[rbase + r] = m * 0.6931471805599453f;
-                    if (p.Li) p.Li[rbase + r] = l;
+                    part[C::O_FLOATS + col + k] = mk;
+                    part[C::O_FLOATS + C::ROWS + col + k] = lk;
+                } else if (row0 + col + k < p.R) {
+                    if (p.Mi) p.Mi[rbase + row0 + col + k] = mk * 0.6931471805599453f;
+                    if (p.Li) p.Li[rbase + row0 + col + k] = lk;
                 }
             }
         }
+    }
 }
 
 // What the merge of a unit across CTAs costs, in tiles of one CTA.
 constexpr unsigned kQ4MergeTiles = 32;
 
 __device__ __forceinline__ float q4_weight(float m, float M) { return m == -INFINITY ? 0.f : ex2_approx(m - M); }
+
+// One thread's share of a merge: the V4 float4 of item idx / 32, lane idx % 32 (q4_emit's order),
+// over parts 0..count-1.  Part i is at first (i = 0), last (i = count - 1) or mid + i * stride.
+template <int D, int NT>
+struct Q4Merged {
+    float4 a[Q4AttnCfg<D, NT>::V4];
+    float M, L;
+    int col, dim;
+    bool stats;                    // this thread also writes the column's M and L
+};
+template <int D, int NT, bool GLOBAL>
+__device__ __forceinline__ Q4Merged<D, NT> q4_merge(int idx, int count, const float* first, const float* mid, size_t stride,
+                                                    const float* last) {
+    using C = Q4AttnCfg<D, NT>;
+    constexpr int U = GLOBAL ? 8 : 4;                                    // parts in flight
+    const int ln = idx & 31, item = idx >> 5;
+    const int e = item & 3, set = (item >> 2) % C::SETS, n = item / (4 * C::SETS);
+    Q4Merged<D, NT> r;
+    r.col = 8 * n + 2 * (ln & 3) + (e & 1);
+    r.dim = q4_dim<D>(set, e, 0, ln >> 2);
+    r.stats = (ln >> 2) == 0 && set == 0 && (e >> 1) == 0;
+    r.M = -INFINITY;
+    r.L = 0.f;
+#pragma unroll
+    for (int v = 0; v < C::V4; ++v) r.a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int st = C::O_FLOATS + r.col, at = item * (C::V4 * 128) + ln * 4;
+#pragma unroll 1
+    for (int i0 = 0; i0 < count; i0 += U) {
+        float m[U], l[U], M = r.M;
+        float4 y[U][C::V4];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            m[i] = -INFINITY;
+            if (i0 + i >= count) continue;
+            const float* part = i0 + i == 0 ? first : i0 + i == count - 1 ? last : mid + (i0 + i) * stride;
+            m[i] = GLOBAL ? __ldcg(part + st) : part[st];
+            l[i] = GLOBAL ? __ldcg(part + st + C::ROWS) : part[st + C::ROWS];
+#pragma unroll
+            for (int v = 0; v < C::V4; ++v) {
+                const float4* src = reinterpret_cast<const float4*>(part + at) + v * 32;
+                y[i][v] = GLOBAL ? __ldcg(src) : *src;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) M = fmaxf(M, m[i]);
+        const float w0 = q4_weight(r.M, M);
+        r.M = M;
+        r.L *= w0;
+#pragma unroll
+        for (int v = 0; v < C::V4; ++v) { r.a[v].x *= w0; r.a[v].y *= w0; r.a[v].z *= w0; r.a[v].w *= w0; }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (i0 + i >= count) continue;
+            const float w = q4_weight(m[i], M);
+            r.L = fmaf(w, l[i], r.L);
+#pragma unroll
+            for (int v = 0; v < C::V4; ++v) {
+                r.a[v].x = fmaf(w, y[i][v].x, r.a[v].x); r.a[v].y = fmaf(w, y[i][v].y, r.a[v].y);
+                r.a[v].z = fmaf(w, y[i][v].z, r.a[v].z); r.a[v].w = fmaf(w, y[i][v].w, r.a[v].w);
+            }
+        }
+    }
+    return r;
+}
+template <int D, int NT>
+__device__ __forceinline__ void q4_write(const Q4AttnParams& p, const Q4Merged<D, NT>& r, int u) {
+    using C = Q4AttnCfg<D, NT>;
+    const int h = p.n_rg == 1 ? u : u / p.n_rg, row = (u - h * p.n_rg) * C::ROWS + r.col;
+    if (row >= p.R) return;
+    const size_t at = static_cast<size_t>(h) * p.R + row;
+    const float inv = r.L == 0.f ? 0.f : 1.0f / r.L;
+#pragma unroll
+    for (int v = 0; v < C::V4; ++v)
+        store_out4(p.O, at * D + r.dim + 4 * v,
+                   make_float4(r.a[v].x * inv, r.a[v].y * inv, r.a[v].z * inv, r.a[v].w * inv), p.out_type);
+    if (r.stats && p.Mi) p.Mi[at] = r.M * 0.6931471805599453f;
+    if (r.stats && p.Li) p.Li[at] = r.L;
+}
 
 template <int D, int NT>
 __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
@@ -489,11 +578,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     __shared__ uint64_t bars[W][STAGES];
     __shared__ int s_abort, s_drop[W], s_last[2];
     __shared__ uint32_t s_valid[W][STAGES];                              // groups copied, 2 bits
-    __shared__ int s_sum[W];
-    __shared__ int s_b[W], s_base[W];
     __shared__ Q4Unit s_ent[2 * W];
-    __shared__ int s_list[2 * W];
-    __shared__ float s_wt[2 * W][C::ROWS], s_mx[2 * W][C::ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* heads = reinterpret_cast<float*>(smem + C::RING_BYTES);
     uint8_t* ring = smem + warp * STAGES * C::STAGE_BYTES;
@@ -504,16 +589,19 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         s_ent[2 * warp].u = s_ent[2 * warp + 1].u = -1;
         fence_mbar_init();
     }
+    __syncthreads();
     grid_dep_launch_dependents();
     grid_dep_wait();
 
-    // ---- the row of tiles: totals, this CTA's share, each warp's first sequence
+    // ---- the row of tiles: totals, this CTA's share, this warp's place (every warp for itself:
+    // lane i counts the tiles of sequences i * per ...)
     const int HR = p.H_kv * p.n_rg;
-    const int per = (p.B + C::THREADS - 1) / C::THREADS;
-    const int b0 = tid * per < p.B ? tid * per : p.B, b1 = b0 + per < p.B ? b0 + per : p.B;
-    int mine = 0;
+    const int per = (p.B + 31) >> 5;
+    const int b0 = lane * per < p.B ? lane * per : p.B, b1 = b0 + per < p.B ? b0 + per : p.B;
     const int nt0 = q4_tiles(q4_len(p, 0));
+    int mine = 0;
     bool same = true;
+#pragma unroll 4
     for (int b = b0; b < b1; ++b) {
         const int nt = q4_tiles(q4_len(p, b));
         mine += nt;
@@ -525,63 +613,46 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
     }
-    if (lane == 31) s_sum[warp] = incl;
-    const bool s_same = __syncthreads_and(same);
-    unsigned total = 0, before = incl - mine;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const unsigned v = s_sum[w];
-        before += w < warp ? v : 0u;
-        total += v;
-    }
-    const unsigned T = total * HR;                                       // < 2^31, the host sees to it
+    const unsigned T = __shfl_sync(0xffffffffu, incl, 31) * HR;          // < 2^31, the host sees to it
     // CTAs that take part: every warp of theirs gets at least a tile.  CTA c has the tiles from
     // c * quot + min(c, rem), warp w of it those from x0 + w * (x1 - x0) / W.
     const unsigned want = (T + W - 1) / W;
     unsigned act = want < gridDim.x ? want : gridDim.x, quot = T / act, rem = T - quot * act;
     // Sequences of one length: whole units to each CTA, if that takes no longer than an even
     // split and the merge across CTAs that it needs.
-    if (s_same) {
-        const unsigned units = p.B * HR, nt = total / p.B, each = (units + gridDim.x - 1) / gridDim.x;
-        if (each * nt <= quot + kQ4MergeTiles) {
-            act = (units + each - 1) / each;
-            quot = each * nt;
+    if (__all_sync(0xffffffffu, same)) {
+        const unsigned units = p.B * HR, each = units <= gridDim.x ? 1 : (units + gridDim.x - 1) / gridDim.x;
+        if (each * nt0 <= quot + kQ4MergeTiles) {
+            act = each == 1 ? units : (units + each - 1) / each;
+            quot = each * nt0;
             rem = 0;
         }
     }
     if (blockIdx.x >= act) return;
     const int x0 = blockIdx.x * quot + (blockIdx.x < rem ? blockIdx.x : rem);
-    int x1 = x0 + quot + (blockIdx.x < rem ? 1 : 0);
-    if (blockIdx.x == act - 1) x1 = T;
+    const int x1 = blockIdx.x == act - 1 ? T : x0 + quot + (blockIdx.x < rem ? 1 : 0);
     const int wq = (x1 - x0) / W, wr = (x1 - x0) % W;
-    auto warp_start = [&](int w) { return x0 + w * wq + (w < wr ? w : wr); };
-    if (mine > 0) {
-        const int lo = before * HR, hi = lo + mine * HR;
-        if (hi > x0 && lo < x1)
-            for (int w = 0; w < W; ++w) {
-                const int y = warp_start(w);
-                if (y < lo || y >= hi) continue;
-                int at = lo, b = b0;
-                for (; b < b1 - 1; ++b) {
-                    const int next = at + q4_tiles(q4_len(p, b)) * HR;
-                    if (y < next) break;
-                    at = next;
-                }
-                s_b[w] = b;
-                s_base[w] = at;
-            }
-    }
-    __syncthreads();
+    const int y0 = x0 + warp * wq + (warp < wr ? warp : wr), y1 = y0 + wq + (warp < wr ? 1 : 0);
 
-    const int y0 = warp_start(warp), y1 = warp_start(warp + 1);
     if (y0 < y1) {
         int y_cur = y0;                                                  // the tile in work
         Q4Cursor cur;
-        cur.b = s_b[warp];
-        cur.len = q4_len(p, cur.b);
-        cur.nt = q4_tiles(cur.len);
         {
-            const unsigned off = y0 - s_base[warp], hr = off / cur.nt;
+            const int lo = (incl - mine) * HR;
+            const bool here = y0 >= lo && y0 < incl * HR;
+            int b = b0, at = lo;
+            if (here)
+                for (; b < b1 - 1; ++b) {
+                    const int next = at + q4_tiles(q4_len(p, b)) * HR;
+                    if (y0 < next) break;
+                    at = next;
+                }
+            const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+            cur.b = __shfl_sync(0xffffffffu, b, from);
+            const unsigned off = y0 - __shfl_sync(0xffffffffu, at, from);
+            cur.len = q4_len(p, cur.b);
+            cur.nt = q4_tiles(cur.len);
+            const unsigned hr = off / cur.nt;
             cur.tile = off - hr * cur.nt;
             cur.h = hr;
             cur.rg = 0;
@@ -629,8 +700,8 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                 }
             }
         };
-        auto move_on = [&]() {
-            win0 = issued;
+        auto move_on = [&](int y) {
+            win0 = y;
             const bool v0 = e0 < static_cast<unsigned>(p.n_blocks), v1 = e1 < static_cast<unsigned>(p.n_blocks);
             const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
             src0 = p.cache + static_cast<uint64_t>(e0 * p.H_kv + (e_at >> 4)) * page_bytes + (e_at & 15u) * C::GROUP;
@@ -639,26 +710,24 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
             valid = (v0 ? 1u : 0u) | (v1 ? 2u : 0u);
             if (win0 + 32 < y1) fetch(win0 + 32);
         };
-        auto issue = [&](int stage) {
-            if (lane == issued - win0) {
-                uint64_t* bar = &bars[warp][stage];
-                uint8_t* dst = ring + stage * C::STAGE_BYTES;
-                s_valid[warp][stage] = valid;
-                mbar_arrive_expect_tx(bar, bytes);
-                if (!paired) {
-                    if (bytes) bulk_g2s(dst, src0, bytes, bar);          // both groups lie in one page
-                } else {
-                    if (valid & 1u) bulk_g2s(dst, src0, C::GROUP, bar);
-                    if (valid & 2u) bulk_g2s(dst + C::GROUP, src1, C::GROUP, bar);
-                }
+        auto issue = [&](int stage) {                                    // by the lane that holds the tile
+            uint64_t* bar = &bars[warp][stage];
+            uint8_t* dst = ring + stage * C::STAGE_BYTES;
+            s_valid[warp][stage] = valid;
+            mbar_arrive_expect_tx(bar, bytes);
+            if (!paired) {
+                if (bytes) bulk_g2s(dst, src0, bytes, bar);              // both groups lie in one page
+            } else {
+                if (valid & 1u) bulk_g2s(dst, src0, C::GROUP, bar);
+                if (valid & 2u) bulk_g2s(dst + C::GROUP, src1, C::GROUP, bar);
             }
-            ++issued;
         };
 
         fetch(y0);
-        move_on();
-#pragma unroll 1
-        for (int i = 0; i < STAGES && issued < y1; ++i) issue(i);
+        move_on(y0);
+        issued = y0 + STAGES < y1 ? y0 + STAGES : y1;
+        if (lane < issued - y0) issue(lane);
+        __syncwarp();
         Q4Warp<D, NT> s;
         int stage = 0;
         uint32_t phase = 0;
@@ -692,8 +761,9 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                 ++y_cur;
                 __syncwarp();
                 if (issued < y1) {
-                    if (issued - win0 == 32) move_on();
-                    issue(stage);
+                    if (issued - win0 == 32) move_on(issued);
+                    if (lane == issued - win0) issue(stage);
+                    ++issued;
                 }
                 if (++stage == STAGES) {
                     stage = 0;
@@ -721,77 +791,38 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     __syncthreads();
 
     // ---- merge the CTA's parts: runs of equal units in the entries' order
-    constexpr int n4 = NT * C::SETS * 4 * C::V4;
-    auto entry = [&](int i) {
-        return i & 1 ? reinterpret_cast<const float*>(smem + (i >> 1) * STAGES * C::STAGE_BYTES)
-                     : heads + (i >> 1) * C::PART_FLOATS;
-    };
+    constexpr int items = NT * C::SETS * 4;
     const Q4Unit mine_u = lane < 2 * W ? s_ent[lane] : Q4Unit{-1, 0, 0};
-    const uint32_t used = __ballot_sync(0xffffffffu, mine_u.u >= 0);
-    if (warp == 0 && mine_u.u >= 0) s_list[__popc(used & ((1u << lane) - 1))] = lane;
-    // Each entry's weight per column, a lane an entry.
-    for (int col = warp; col < C::ROWS; col += W) {
-        const float m = mine_u.u >= 0 ? entry(lane)[C::O_FLOATS + col] : -INFINITY;
-        for (uint32_t todo = used; todo;) {
-            const uint32_t run = __ballot_sync(0xffffffffu, mine_u.u == __shfl_sync(0xffffffffu, mine_u.u, __ffs(todo) - 1));
-            todo &= ~run;
-            const bool in = (run >> lane) & 1u;
-            float M = in ? m : -INFINITY;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            if (in) {
-                s_wt[lane][col] = q4_weight(m, M);
-                s_mx[lane][col] = M;
-            }
-        }
-    }
-    __syncthreads();
     int cross_u[2] = {-1, -1}, cross_first[2] = {0, 0}, cross_n[2] = {0, 0};
-    int at = 0;
-    for (uint32_t todo = used; todo;) {
+    for (uint32_t todo = __ballot_sync(0xffffffffu, mine_u.u >= 0); todo;) {
         const int lead = __ffs(todo) - 1;
         const int u = __shfl_sync(0xffffffffu, mine_u.u, lead);
         const int us = __shfl_sync(0xffffffffu, mine_u.start, lead), unt = __shfl_sync(0xffffffffu, mine_u.nt, lead);
         const uint32_t run = __ballot_sync(0xffffffffu, mine_u.u == u);
-        const int from = at, to = at + __popc(run);
-        at = to;
         todo &= ~run;
+        // A unit's first part here is in slot `lead`; the others are the last parts (odd slots) of
+        // the warps that follow, but for the run's end, which may be a head (even) slot.
+        const int count = __popc(run), end = 31 - __clz(run);
+        auto entry = [&](int f) {
+            return reinterpret_cast<const float*>(f & 1 ? smem + (f >> 1) * (STAGES * C::STAGE_BYTES)
+                                                        : smem + C::RING_BYTES + (f >> 1) * (C::PART_FLOATS * 4));
+        };
         const bool inside = us >= x0 && us + unt <= x1;
         const int slot = us >= x0 ? 1 : 0;
         float* out = p.parts + (static_cast<size_t>(blockIdx.x) * 2 + slot) * C::PART_FLOATS;
-        const int row0 = (u % p.n_rg) * C::ROWS;
-        const size_t rbase = static_cast<size_t>(u / p.n_rg) * p.R;
 #pragma unroll 1
-        for (int idx = tid; idx < n4 * 32; idx += C::THREADS) {
-            const int ln = idx & 31, q4 = idx >> 5, v = q4 % C::V4, item = q4 / C::V4;
-            const int e = item & 3, set = (item >> 2) % C::SETS, n = item / (4 * C::SETS);
-            const int col = 8 * n + 2 * (ln & 3) + (e & 1), r = row0 + col;
-            float L = 0.f;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int i = from; i < to; ++i) {
-                const int f = s_list[i];
-                const float* part = entry(f);
-                const float w = s_wt[f][col];
-                const float4 y = reinterpret_cast<const float4*>(part)[q4 * 32 + ln];
-                L = fmaf(w, part[C::O_FLOATS + C::ROWS + col], L);
-                a.x = fmaf(w, y.x, a.x); a.y = fmaf(w, y.y, a.y); a.z = fmaf(w, y.z, a.z); a.w = fmaf(w, y.w, a.w);
-            }
-            const bool stats = (ln >> 2) == 0 && set == 0 && v == 0 && (e >> 1) == 0;
-            const float M = s_mx[lead][col];
+        for (int idx = tid; idx < items * 32; idx += C::THREADS) {
+            const Q4Merged<D, NT> r = q4_merge<D, NT, false>(idx, count, entry(lead), entry(lead | 1),
+                                                             STAGES * C::STAGE_BYTES / 4, entry(end));
             if (inside) {
-                const float inv = L == 0.f ? 0.f : 1.0f / L;
-                if (r < p.R) {
-                    store_out4(p.O, (rbase + r) * D + q4_dim<D>(set, e, v, ln >> 2),
-                               make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv), p.out_type);
-                    if (stats && p.Mi) p.Mi[rbase + r] = M * 0.6931471805599453f;
-                    if (stats && p.Li) p.Li[rbase + r] = L;
-                }
+                q4_write(p, r, u);
             } else {
-                reinterpret_cast<float4*>(out)[q4 * 32 + ln] = a;
-                if (stats) {
-                    out[C::O_FLOATS + col] = M;
-                    out[C::O_FLOATS + C::ROWS + col] = L;
+                float4* o = reinterpret_cast<float4*>(out) + (idx >> 5) * (C::V4 * 32) + (idx & 31);
+#pragma unroll
+                for (int v = 0; v < C::V4; ++v) o[v * 32] = r.a[v];
+                if (r.stats) {
+                    out[C::O_FLOATS + r.col] = r.M;
+                    out[C::O_FLOATS + C::ROWS + r.col] = r.L;
                 }
             }
         }
@@ -826,59 +857,16 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         }
     }
     __syncthreads();
-    float* wm = reinterpret_cast<float*>(smem);                          // [parts][ROWS] m, then weights; [parts][ROWS] l; totals
 #pragma unroll 1
     for (int k = 0; k < 2; ++k) {
         if (!s_last[k]) continue;
-        const int nparts = k ? cross_n[1] : cross_n[0], cf = k ? cross_first[1] : cross_first[0], u = k ? cross_u[1] : cross_u[0];
-        float* wl = wm + nparts * C::ROWS;
-        float* tot = wl + nparts * C::ROWS;                              // M, L per column
-        auto part = [&](int i) { return p.parts + (static_cast<size_t>(cf + i) * 2 + (i == 0 ? 1 : 0)) * C::PART_FLOATS; };
-        __syncthreads();
-        for (int i = tid; i < nparts * C::ROWS; i += C::THREADS) {
-            const float* src = part(i / C::ROWS) + C::O_FLOATS + i % C::ROWS;
-            wm[i] = __ldcg(src);
-            wl[i] = __ldcg(src + C::ROWS);
-        }
-        __syncthreads();
-        for (int col = warp; col < C::ROWS; col += W) {
-            float M = -INFINITY, L = 0.f;
-            for (int i = lane; i < nparts; i += 32) M = fmaxf(M, wm[i * C::ROWS + col]);
-            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            for (int i = lane; i < nparts; i += 32) {
-                const float w = q4_weight(wm[i * C::ROWS + col], M);
-                wm[i * C::ROWS + col] = w;
-                L = fmaf(w, wl[i * C::ROWS + col], L);
-            }
-            for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-            if (lane == 0) {
-                tot[2 * col] = M;
-                tot[2 * col + 1] = L;
-            }
-        }
-        __syncthreads();
-        const int row0 = (u % p.n_rg) * C::ROWS;
-        const size_t rbase = static_cast<size_t>(u / p.n_rg) * p.R;
-        for (int idx = tid; idx < n4 * 32; idx += C::THREADS) {
-            const int ln = idx & 31, q4 = idx >> 5, v = q4 % C::V4, item = q4 / C::V4;
-            const int e = item & 3, set = (item >> 2) % C::SETS, n = item / (4 * C::SETS);
-            const int col = 8 * n + 2 * (ln & 3) + (e & 1), r = row0 + col;
-            if (r >= p.R) continue;
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int i = 0; i < nparts; ++i) {
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(part(i)) + q4 * 32 + ln);
-                const float w = wm[i * C::ROWS + col];
-                a.x = fmaf(w, y.x, a.x); a.y = fmaf(w, y.y, a.y); a.z = fmaf(w, y.z, a.z); a.w = fmaf(w, y.w, a.w);
-            }
-            const float L = tot[2 * col + 1], inv = L == 0.f ? 0.f : 1.0f / L;
-            store_out4(p.O, (rbase + r) * D + q4_dim<D>(set, e, v, ln >> 2),
-                       make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv), p.out_type);
-            if ((ln >> 2) == 0 && set == 0 && v == 0 && (e >> 1) == 0) {
-                if (p.Mi) p.Mi[rbase + r] = tot[2 * col] * 0.6931471805599453f;
-                if (p.Li) p.Li[rbase + r] = L;
-            }
-        }
+        const int cf = k ? cross_first[1] : cross_first[0], u = k ? cross_u[1] : cross_u[0];
+        const int count = k ? cross_n[1] : cross_n[0];
+        const float* mid = p.parts + static_cast<size_t>(cf) * 2 * C::PART_FLOATS;   // its first CTA's second slot, then first slots
+#pragma unroll 1
+        for (int idx = tid; idx < items * 32; idx += C::THREADS)
+            q4_write(p, q4_merge<D, NT, true>(idx, count, mid + C::PART_FLOATS, mid, 2 * C::PART_FLOATS,
+                                              mid + (count - 1) * 2 * C::PART_FLOATS), u);
     }
 }
 
