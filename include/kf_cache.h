@@ -46,17 +46,17 @@ extern "C" {
 /* Quantises k and v (both [B, H_kv, S, D] by element strides, head dimension contiguous)
  * into the cache: token (b, s) goes to slot slots[b * S + s].  A slot outside
  * [0, n_blocks * block_size) is skipped (padding: -1).  If one slot is named twice, either
- * token's K and V may end there.  Strides: multiples of 8, >= 0.  B * S == 0 is a no-op. */
+ * token's K and V may end there.  strides: 6 values in host memory, the batch, head and token
+ * strides of k, then of v; multiples of 8, >= 0 (of a dimension of one element: any).
+ * B * S == 0 is a no-op. */
 int kf_kv_write_q4(const void* k, const void* v, void* cache, const int* slots, int B, int S, int H_kv, int D,
-                   int n_blocks, int block_size, long long k_stride_b, long long k_stride_h, long long k_stride_s,
-                   long long v_stride_b, long long v_stride_h, long long v_stride_s, unsigned flags, void* stream);
+                   int n_blocks, int block_size, const long long* strides, unsigned flags, void* stream);
 
 /* Reads slots back into k and v (layout and strides as kf_kv_write_q4, outputs distinct
  * and without overlap): rnd(s * (n - z)), one rounding.  A slot outside
  * [0, n_blocks * block_size) reads zeros. */
 int kf_kv_read_q4(const void* cache, const int* slots, void* k, void* v, int B, int S, int H_kv, int D,
-                  int n_blocks, int block_size, long long k_stride_b, long long k_stride_h, long long k_stride_s,
-                  long long v_stride_b, long long v_stride_h, long long v_stride_s, unsigned flags, void* stream);
+                  int n_blocks, int block_size, const long long* strides, unsigned flags, void* stream);
 
 /* Attention over the cache: O[b, h, i] = softmax_j(scale * q . k_j) v_j over the keys
  * j < seq_lens[b] of sequence b, whose logical block n is pool block

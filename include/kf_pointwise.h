@@ -66,14 +66,14 @@ int kf_rope(void* q, void* k, const int* positions, const float* inv_freq, int B
  * any input.  q_weight / k_weight [D]; NULL: ones.  positions, inv_freq, theta, rot_dim
  * and KF_ROPE_GPTJ as kf_rope; rot_dim == 0: no rotation.  rot_scale multiplies cos and sin
  * (the attention factor of long-context settings; 1 otherwise).
- * D: a multiple of 16, at most 512.  Strides: multiples of 8, >= 0.
+ * strides: 12 values in host memory, the batch, head and token strides of q, k, q_out and
+ * k_out in this order; multiples of 8, >= 0 (of a dimension of one element: any).
+ * D: a multiple of 16, at most 512.
  * k may be NULL when H_kv == 0.  B * S == 0 is a no-op. */
 int kf_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, void* q_out,
                     void* k_out, const int* positions, const float* inv_freq, int B, int S, int H_q, int H_kv, int D,
-                    int rot_dim, float theta, float rot_scale, float eps, long long q_stride_b, long long q_stride_h,
-                    long long q_stride_s, long long k_stride_b, long long k_stride_h, long long k_stride_s,
-                    long long qo_stride_b, long long qo_stride_h, long long qo_stride_s, long long ko_stride_b,
-                    long long ko_stride_h, long long ko_stride_s, unsigned flags, void* stream);
+                    int rot_dim, float theta, float rot_scale, float eps, const long long* strides, unsigned flags,
+                    void* stream);
 
 /* SwiGLU on the fused gate/up projection output gate_up [rows, 2 * inter]
  * (gate columns first): out[r, j] = rnd(rnd(silu(g)) * u) with

@@ -132,11 +132,11 @@ def lib():
     L.kf_rmsnorm.restype = I
     L.kf_rope.argtypes = [P, P, P, P, I, I, I, I, I, I, F, LL, LL, LL, LL, LL, LL, U, P]
     L.kf_rope.restype = I
-    L.kf_qk_norm_rope.argtypes = [P] * 8 + [I] * 6 + [F] * 3 + [LL] * 12 + [U, P]
+    L.kf_qk_norm_rope.argtypes = [P] * 8 + [I] * 6 + [F] * 3 + [P, U, P]
     L.kf_qk_norm_rope.restype = I
-    L.kf_kv_write_q4.argtypes = [P] * 4 + [I] * 6 + [LL] * 6 + [U, P]
+    L.kf_kv_write_q4.argtypes = [P] * 4 + [I] * 6 + [P, U, P]
     L.kf_kv_write_q4.restype = I
-    L.kf_kv_read_q4.argtypes = [P] * 4 + [I] * 6 + [LL] * 6 + [U, P]
+    L.kf_kv_read_q4.argtypes = [P] * 4 + [I] * 6 + [P, U, P]
     L.kf_kv_read_q4.restype = I
     L.kf_attn_fwd_paged_q4.argtypes = [P] * 7 + [I] * 8 + [F, U, P, Z, P]
     L.kf_attn_fwd_paged_q4.restype = I
@@ -154,6 +154,30 @@ def lib():
 def check(rc: int, what: str = "") -> None:
     if rc != KF_OK:
         raise KFError(rc, what)
+
+
+class CallPlans:
+    """Argument lists that a wrapper worked out for tensors of one set of shapes, strides, types and
+    devices (its key), so that a decode loop pays for the checks of a call's form once.  Pointers and
+    values are never part of a plan."""
+
+    def __init__(self, limit: int = 512):
+        self._plans, self._limit = {}, limit
+
+    def get(self, key):
+        return self._plans.get(key)
+
+    def put(self, key, plan):
+        if len(self._plans) >= self._limit:
+            self._plans.clear()
+        self._plans[key] = plan
+        return plan
+
+
+def strides_arg(*strides):
+    """A host array of strides for the C ABI, and the pointer to it."""
+    a = (ctypes.c_longlong * len(strides))(*strides)
+    return a, ctypes.addressof(a)
 
 
 def on_device(index: int, fn, what: str, *args) -> None:

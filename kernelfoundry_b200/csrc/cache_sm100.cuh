@@ -25,114 +25,195 @@ struct Q4 {
 constexpr uint32_t kQ4BadRow = 0x7FC00000u;                 // word of a row with a NaN or an infinity
 
 __device__ __forceinline__ float q4_scale(uint32_t w) { return __uint_as_float(w & 0xFFFFFF00u); }
-// The zero point as a float: 2^23 + z is exact, so the subtraction leaves z.
-__device__ __forceinline__ float q4_zero(uint32_t w) { return __uint_as_float(0x4B000000u | (w & 15u)) - 8388608.0f; }
 
-// Parameter word of a row from its extremes (lo <= 0 <= hi) and the reciprocal scale.
-__device__ __forceinline__ uint32_t q4_params(float lo, float hi, bool finite, float* inv, float* zp) {
+// Parameter word of a row from its extremes (lo <= 0 <= hi, NaN if the row has one) and what
+// the codes need: the reciprocal scale and the zero point (both 0 for a spoiled row).
+__device__ __forceinline__ uint32_t q4_params(float lo, float hi, float* inv, float* zp) {
     const float c = 1.0f / 15.0f;
     float s = __fsub_rn(__fmul_rn(hi, c), __fmul_rn(lo, c));
-    s = __uint_as_float((__float_as_uint(s) + 0x80u) & 0xFFFFFF00u);
-    if (!(s >= 7.888609052210118e-31f)) s = 0.0f;           // 2^-100: keeps 1/s finite
-    *inv = s == 0.0f ? 0.0f : __frcp_rn(s);
-    *zp = fminf(fmaxf(rintf(__fmul_rn(-lo, *inv)), 0.0f), 15.0f);
-    if (!finite) {
-        *inv = 0.0f;
-        *zp = 0.0f;
+    if (!(fabsf(s) <= 3.402823466e38f)) {                   // finite exactly when the row is
+        *inv = *zp = 0.0f;
         return kQ4BadRow;
     }
+    s = __uint_as_float((__float_as_uint(s) + 0x80u) & 0xFFFFFF00u);
+    if (s < 7.888609052210118e-31f) s = 0.0f;               // 2^-100: keeps 1/s finite
+    *inv = s == 0.0f ? 0.0f : __frcp_rn(s);
+    *zp = fminf(fmaxf(rintf(__fmul_rn(-lo, *inv)), 0.0f), 15.0f);
     return __float_as_uint(s) | static_cast<uint32_t>(*zp);
 }
 
-__device__ __forceinline__ uint32_t q4_code(float x, float inv, float zp) {
-    return static_cast<uint32_t>(fminf(fmaxf(__fadd_rn(rintf(__fmul_rn(x, inv)), zp), 0.0f), 15.0f));
+// Eight codes, clamp(rint(x * inv) + zp, 0, 15), in a word.  Adding 1.5 * 2^23 rounds to an integer
+// (ties to even); the clamp is taken around it, and the nibbles are put together by exact FMAs.
+__device__ __forceinline__ uint32_t q4_codes8(const float (&x)[8], float inv, float zp) {
+    const float m = 12582912.0f, lo = m - zp, hi = lo + 15.0f;
+    float n[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        n[e] = __fadd_rn(fminf(fmaxf(__fadd_rn(__fmul_rn(x[e], inv), m), lo), hi), -lo);
+    float h[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        h[i] = fmaf(fmaf(n[4 * i + 3], 16.0f, n[4 * i + 2]), 256.0f, fmaf(n[4 * i + 1], 16.0f, n[4 * i]));
+    return static_cast<uint32_t>(h[0]) | static_cast<uint32_t>(h[1]) << 16;
+}
+
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 
 struct Q4IoParams {
     uint8_t* cache;
     const int* slots;             // [B, S]
-    uint16_t* k;
-    uint16_t* v;
-    long long k_sb, k_sh, k_ss;   // element strides
+    uint4* k;
+    uint4* v;
+    long long k_sb, k_sh, k_ss;   // strides in 16-byte vectors
     long long v_sb, v_sh, v_ss;
-    int B, S, H;
+    long long n_tokens;           // B * S
+    int S, H;
     int bs_log2;                  // log2(block_size)
+    int TPB;                      // tokens per block
+    int splits, rows_per_split;   // blocks per token group, and their rows (K and V of each head) of it
     long long n_slots;            // n_blocks * block_size
 };
 
-// Byte address of the group that holds `slot` of head h.
+constexpr int kQ4IoTokens = 16;                            // the largest TPB
+
+// Both kernels below are bound by HBM.  A block takes a few tokens (their slots and offsets are
+// looked up once, in shared memory) and all their rows, K and V of each head; a thread has UNR
+// rows in flight.  Rows of one token are neighbours in the 16-bit tensors ([B, S, H, D]) or
+// (token by token) in their head ([B, H, S, D]): either way every access is whole sectors.
+struct Q4Tokens {
+    long long k[kQ4IoTokens], v[kQ4IoTokens];              // offsets in the 16-bit tensors, vectors
+    long long group[kQ4IoTokens];                          // byte offset of head 0's group; -1: no such slot
+    int row[kQ4IoTokens];                                  // row in it
+};
+
 template <int D>
-__device__ __forceinline__ uint8_t* q4_group(uint8_t* cache, long long slot, int h, int H, int bs_log2) {
-    const long long block = slot >> bs_log2;
-    const long long groups = 1ll << (bs_log2 - 4);
-    return cache + ((block * H + h) * groups + ((slot >> 4) & (groups - 1))) * Q4<D>::GROUP;
+__device__ __forceinline__ int q4_tokens(const Q4IoParams& p, Q4Tokens& tok, long long tok0) {
+    const int n = p.n_tokens - tok0 < p.TPB ? static_cast<int>(p.n_tokens - tok0) : p.TPB;
+    const int tid = threadIdx.x;
+    if (tid < n) {
+        const long long t = tok0 + tid, b = t / p.S, s = t - b * p.S;
+        const long long slot = p.slots[t];
+        const long long groups = 1ll << (p.bs_log2 - 4);
+        tok.k[tid] = b * p.k_sb + s * p.k_ss;
+        tok.v[tid] = b * p.v_sb + s * p.v_ss;
+        tok.group[tid] = slot < 0 || slot >= p.n_slots
+                             ? -1 : ((slot >> p.bs_log2) * p.H * groups + ((slot >> 4) & (groups - 1))) * Q4<D>::GROUP;
+        tok.row[tid] = slot & 15;
+    }
+    __syncthreads();
+    return n;
 }
 
-// One warp per (token, head, K or V) row; a lane holds D / 32 neighbouring dims.
+// A row belongs to D / 16 threads with the vectors u and u + D / 16: a store of their words is a
+// whole sector.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) q4_write_kernel(const Q4IoParams p) {
-    constexpr int N = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long rows = 2ll * p.B * p.S * p.H;
-    for (long long r = (blockIdx.x * 256ll + threadIdx.x) >> 5; r < rows; r += gridDim.x * 8ll) {
-        const bool is_v = r & 1;
-        const int h = static_cast<int>((r >> 1) % p.H);
-        const long long tok = (r >> 1) / p.H;
-        const long long slot = p.slots[tok];
-        if (slot < 0 || slot >= p.n_slots) continue;
-        const long long b = tok / p.S, s = tok % p.S;
-        const uint16_t* src = is_v ? p.v + b * p.v_sb + h * p.v_sh + s * p.v_ss : p.k + b * p.k_sb + h * p.k_sh + s * p.k_ss;
-        float x[N], lo = 0.f, hi = 0.f;
-        bool fin = true;
+    constexpr int GS = D / 16, RG = 256 / GS, UNR = 4;
+    __shared__ Q4Tokens tok;
+    const int tid = threadIdx.x, u = tid % GS, H2 = 2 * p.H, split = blockIdx.x % p.splits;
+    const int n = q4_tokens<D>(p, tok, static_cast<long long>(blockIdx.x / p.splits) * p.TPB);
+    const int end = min((split + 1) * p.rows_per_split, n * H2);
+    const size_t head = static_cast<size_t>(Q4<D>::GROUP) << (p.bs_log2 - 4);   // bytes from a head to the next
+    int row = split * p.rows_per_split + tid / GS;
+    int t = row / H2, r = row - t * H2;                                  // token, row of it: K of each head, then V
+    for (; row - tid / GS < end; row += UNR * RG) {
+        uint4 x4[UNR][2];
+        uint8_t* dst[UNR];
+        int at[UNR];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            x[i] = to_f32<BF16>(src[lane * N + i]);
-            fin = fin && isfinite(x[i]);
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
+        for (int i = 0; i < UNR; ++i) {
+            dst[i] = nullptr;
+            x4[i][0] = x4[i][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (row + i * RG < end && tok.group[t] >= 0) {
+                const bool is_v = r >= p.H;
+                const int h = is_v ? r - p.H : r;
+                const uint4* src = is_v ? p.v + tok.v[t] + h * p.v_sh : p.k + tok.k[t] + h * p.k_sh;
+                x4[i][0] = ld_stream(src + u);
+                x4[i][1] = ld_stream(src + u + GS);
+                dst[i] = p.cache + tok.group[t] + h * head + (is_v ? Q4<D>::V_CODES : 0);
+                at[i] = tok.row[t];
+                if (is_v) at[i] |= 16;
+            }
+            for (r += RG; r >= H2; r -= H2) ++t;
         }
-        for (int o = 16; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-        fin = __all_sync(0xffffffffu, fin);
-        float inv, zp;
-        const uint32_t word = q4_params(lo, hi, fin, &inv, &zp);
-        uint8_t* grp = q4_group<D>(p.cache, slot, h, p.H, p.bs_log2);
-        uint8_t* dst = grp + (is_v ? Q4<D>::V_CODES : 0) + (slot & 15) * Q4<D>::ROW + lane * (N / 2);
 #pragma unroll
-        for (int i = 0; i < N; i += 2)
-            dst[i / 2] = fin ? static_cast<uint8_t>(q4_code(x[i], inv, zp) | (q4_code(x[i + 1], inv, zp) << 4)) : 0;
-        if (lane == 0)
-            reinterpret_cast<uint32_t*>(grp + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS))[slot & 15] = word;
+        for (int i = 0; i < UNR; ++i) {
+            float x[2][8], lo = 0.f, hi = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                unpack8<BF16>(x4[i][c], x[c]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    lo = fminf(lo, x[c][e]);
+                    hi = fmax_nan(hi, x[c][e]);
+                }
+            }
+#pragma unroll
+            for (int o = GS / 2; o > 0; o >>= 1) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            if (!dst[i]) continue;
+            float inv, zp;
+            const uint32_t word = q4_params(lo, hi, &inv, &zp);
+            const int rr = at[i] & 15;
+            uint32_t* w = reinterpret_cast<uint32_t*>(dst[i] + rr * Q4<D>::ROW);
+            if (word == kQ4BadRow) {
+                w[u] = w[u + GS] = 0u;
+            } else {
+                w[u] = q4_codes8(x[0], inv, zp);
+                w[u + GS] = q4_codes8(x[1], inv, zp);
+            }
+            if (u == 0)
+                reinterpret_cast<uint32_t*>(dst[i] + (at[i] & 16 ? Q4<D>::V_WORDS - Q4<D>::V_CODES : Q4<D>::K_WORDS))[rr] = word;
+        }
     }
 }
 
+// A row belongs to D / 8 threads with a word (8 codes, one 16-byte vector) each.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) q4_read_kernel(const Q4IoParams p) {
-    constexpr int N = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long rows = 2ll * p.B * p.S * p.H;
-    for (long long r = (blockIdx.x * 256ll + threadIdx.x) >> 5; r < rows; r += gridDim.x * 8ll) {
-        const bool is_v = r & 1;
-        const int h = static_cast<int>((r >> 1) % p.H);
-        const long long tok = (r >> 1) / p.H;
-        const long long slot = p.slots[tok];
-        const long long b = tok / p.S, s = tok % p.S;
-        uint16_t* dst = is_v ? p.v + b * p.v_sb + h * p.v_sh + s * p.v_ss : p.k + b * p.k_sb + h * p.k_sh + s * p.k_ss;
-        float sc = 0.f, zp = 0.f;
-        const uint8_t* src = nullptr;
-        if (slot >= 0 && slot < p.n_slots) {
-            const uint8_t* grp = q4_group<D>(p.cache, slot, h, p.H, p.bs_log2);
-            const uint32_t w = reinterpret_cast<const uint32_t*>(grp + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS))[slot & 15];
-            sc = q4_scale(w);
-            zp = q4_zero(w);
-            src = grp + (is_v ? Q4<D>::V_CODES : 0) + (slot & 15) * Q4<D>::ROW + lane * (N / 2);
+    constexpr int GS = D / 8, RG = 256 / GS, UNR = 8;
+    __shared__ Q4Tokens tok;
+    const int tid = threadIdx.x, u = tid % GS, H2 = 2 * p.H, split = blockIdx.x % p.splits;
+    const int n = q4_tokens<D>(p, tok, static_cast<long long>(blockIdx.x / p.splits) * p.TPB);
+    const int end = min((split + 1) * p.rows_per_split, n * H2);
+    const size_t head = static_cast<size_t>(Q4<D>::GROUP) << (p.bs_log2 - 4);
+    int row = split * p.rows_per_split + tid / GS;
+    int t = row / H2, r = row - t * H2;
+    for (; row < end; row += UNR * RG) {
+        uint32_t w[UNR], word[UNR];
+        uint4* dst[UNR];
+#pragma unroll
+        for (int i = 0; i < UNR; ++i) {
+            dst[i] = nullptr;
+            w[i] = word[i] = 0u;
+            if (row + i * RG < end) {
+                const bool is_v = r >= p.H;
+                const int h = is_v ? r - p.H : r;
+                dst[i] = (is_v ? p.v + tok.v[t] + h * p.v_sh : p.k + tok.k[t] + h * p.k_sh) + u;
+                if (tok.group[t] >= 0) {
+                    const uint8_t* g = p.cache + tok.group[t] + h * head;
+                    const int rr = tok.row[t];
+                    w[i] = __ldg(reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW) + u);
+                    word[i] = __ldg(reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS)) + rr);
+                }
+            }
+            for (r += RG; r >= H2; r -= H2) ++t;
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t n = src ? (src[i / 2] >> (4 * (i & 1))) & 15u : 0u;
-            dst[lane * N + i] = from_f32<BF16>(sc * (static_cast<float>(n) - zp));
+        for (int i = 0; i < UNR; ++i) {
+            if (!dst[i]) continue;
+            const float s = q4_scale(word[i]), z = __uint_as_float(0x4B000000u | (word[i] & 15u));
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] = s * (__uint_as_float(0x4B000000u | ((w[i] >> (4 * e)) & 15u)) - z);   // 2^23 + n, 2^23 + z: exact
+            st_stream(dst[i], pack8<BF16>(x));
         }
     }
 }

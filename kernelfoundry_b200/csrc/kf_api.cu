@@ -1335,12 +1335,27 @@ void drop_unused_strides(int B, int H, int S, long long& b, long long& h, long l
 }
 
 template <bool BF16, bool NEOX>
-int qk_norm_rope_t(const kf::QkNormRopeParams& p, cudaStream_t s) {
-    int grid = 0;
-    int rc = pw_grid<kf::qk_norm_rope_kernel<BF16, NEOX>>(256, (p.n_tokens * (p.H_q + p.H_kv) + 7) / 8, &grid);
-    if (rc != KF_OK) return rc;
+int qk_norm_rope_t(const kf::QkNormRopeParams& p, unsigned grid, cudaStream_t s) {
     kf::qk_norm_rope_kernel<BF16, NEOX><<<grid, 256, 0, s>>>(p);
     return launch_status();
+}
+
+// Blocks of `per` tokens with `rows` rows each (a block passes over `group` rows at a time): as
+// many tokens as leave two blocks an SM, and where even single tokens are fewer than that, the
+// rows of a token are split.
+void token_blocks(long long n_tokens, int rows, int group, int max_per, int sm_count, int* per, int* splits,
+                  int* rows_per_split, long long* blocks) {
+    int t = max_per;
+    while (t > 1 && (n_tokens + t - 1) / t < 2ll * sm_count) t >>= 1;
+    *per = t;
+    const int passes = (t * rows + group - 1) / group;
+    long long sp = t > 1 ? 1 : 2ll * sm_count / (n_tokens > 0 ? n_tokens : 1);
+    if (sp > passes) sp = passes;
+    if (sp < 1) sp = 1;
+    const int pps = (passes + static_cast<int>(sp) - 1) / static_cast<int>(sp);
+    *splits = (passes + pps - 1) / pps;
+    *rows_per_split = pps * group;
+    *blocks = (n_tokens + t - 1) / t * *splits;
 }
 
 }  // namespace
@@ -1431,10 +1446,8 @@ int kf_rope(void* q, void* k, const int* positions, const float* inv_freq, int B
 
 int kf_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, void* q_out,
                     void* k_out, const int* positions, const float* inv_freq, int B, int S, int H_q, int H_kv, int D,
-                    int rot_dim, float theta, float rot_scale, float eps, long long q_stride_b, long long q_stride_h,
-                    long long q_stride_s, long long k_stride_b, long long k_stride_h, long long k_stride_s,
-                    long long qo_stride_b, long long qo_stride_h, long long qo_stride_s, long long ko_stride_b,
-                    long long ko_stride_h, long long ko_stride_s, unsigned flags, void* stream) {
+                    int rot_dim, float theta, float rot_scale, float eps, const long long* strides, unsigned flags,
+                    void* stream) {
     if (flags & ~static_cast<unsigned>(KF_PW_BF16 | KF_ROPE_GPTJ)) return KF_ERR_INVALID_ARG;
     const bool neox = !(flags & KF_ROPE_GPTJ);
     if (B < 0 || S < 0 || H_q < 0 || H_kv < 0 || H_q > 65535 || H_kv > 65535 || H_q + H_kv < 1) return KF_ERR_INVALID_ARG;
@@ -1444,45 +1457,55 @@ int kf_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
     if (!(eps >= 0.f) || !std::isfinite(eps) || !std::isfinite(rot_scale)) return KF_ERR_INVALID_ARG;
     const long long n_tokens = static_cast<long long>(B) * S;
     if (n_tokens == 0) return KF_OK;
-    drop_unused_strides(B, H_q, S, q_stride_b, q_stride_h, q_stride_s);
-    drop_unused_strides(B, H_q, S, qo_stride_b, qo_stride_h, qo_stride_s);
-    drop_unused_strides(B, H_kv, S, k_stride_b, k_stride_h, k_stride_s);
-    drop_unused_strides(B, H_kv, S, ko_stride_b, ko_stride_h, ko_stride_s);
-    if (H_q > 0 && (!q || !q_out || !strides_ok(q_stride_b, q_stride_h, q_stride_s) ||
-                    !strides_ok(qo_stride_b, qo_stride_h, qo_stride_s)))
-        return KF_ERR_INVALID_ARG;
-    if (H_kv > 0 && (!k || !k_out || !strides_ok(k_stride_b, k_stride_h, k_stride_s) ||
-                     !strides_ok(ko_stride_b, ko_stride_h, ko_stride_s)))
-        return KF_ERR_INVALID_ARG;
+    if (!strides) return KF_ERR_INVALID_ARG;
+    long long st[12];
+    for (int i = 0; i < 4; ++i) {
+        const int H = i & 1 ? H_kv : H_q;
+        for (int j = 0; j < 3; ++j) st[3 * i + j] = strides[3 * i + j];
+        drop_unused_strides(B, H, S, st[3 * i], st[3 * i + 1], st[3 * i + 2]);
+        if (H > 0 && !strides_ok(st[3 * i], st[3 * i + 1], st[3 * i + 2])) return KF_ERR_INVALID_ARG;
+    }
+    if ((H_q > 0 && (!q || !q_out)) || (H_kv > 0 && (!k || !k_out))) return KF_ERR_INVALID_ARG;
     if ((H_q > 0 && (!aligned16(q) || !aligned16(q_out) || !aligned16(q_weight))) ||
         (H_kv > 0 && (!aligned16(k) || !aligned16(k_out) || !aligned16(k_weight))))
         return KF_ERR_MISALIGNED;
+    DeviceInfo* di = nullptr;
+    const int rc = device_info(&di);
+    if (rc != KF_OK) return rc;
     kf::QkNormRopeParams p;
-    p.q = static_cast<const uint16_t*>(q);
-    p.k = static_cast<const uint16_t*>(k);
-    p.qo = static_cast<uint16_t*>(q_out);
-    p.ko = static_cast<uint16_t*>(k_out);
-    p.qw = static_cast<const uint16_t*>(q_weight);
-    p.kw = static_cast<const uint16_t*>(k_weight);
+    p.q = static_cast<const uint4*>(q);
+    p.k = static_cast<const uint4*>(k);
+    p.qo = static_cast<uint4*>(q_out);
+    p.ko = static_cast<uint4*>(k_out);
+    p.qw = static_cast<const uint4*>(q_weight);
+    p.kw = static_cast<const uint4*>(k_weight);
     p.pos = positions;
     p.inv_freq = inv_freq;
-    p.q_sb = q_stride_b; p.q_sh = q_stride_h; p.q_ss = q_stride_s;
-    p.k_sb = k_stride_b; p.k_sh = k_stride_h; p.k_ss = k_stride_s;
-    p.qo_sb = qo_stride_b; p.qo_sh = qo_stride_h; p.qo_ss = qo_stride_s;
-    p.ko_sb = ko_stride_b; p.ko_sh = ko_stride_h; p.ko_ss = ko_stride_s;
+    p.q_sb = st[0] / 8; p.q_sh = st[1] / 8; p.q_ss = st[2] / 8;
+    p.k_sb = st[3] / 8; p.k_sh = st[4] / 8; p.k_ss = st[5] / 8;
+    p.qo_sb = st[6] / 8; p.qo_sh = st[7] / 8; p.qo_ss = st[8] / 8;
+    p.ko_sb = st[9] / 8; p.ko_sh = st[10] / 8; p.ko_ss = st[11] / 8;
     p.n_tokens = n_tokens;
     p.S = S;
     p.H_q = H_q;
     p.H_kv = H_kv;
     p.D = D;
     p.rot_dim = rot_dim;
+    p.GS = 1;
+    while (p.GS < D / 16) p.GS <<= 1;
+    long long blocks = 0;
+    token_blocks(n_tokens, H_q + H_kv, 256 / p.GS, kf::kQkNormRopeTokens, di->sm_count, &p.TPB, &p.splits,
+                 &p.rows_per_split, &blocks);
+    if (blocks >= (1ll << 31)) return KF_ERR_INVALID_ARG;
     p.eps = eps;
     p.rot_scale = rot_scale;
+    p.inv_D = 1.0f / static_cast<float>(D);
     p.log2_theta = inv_freq || rot_dim == 0 ? 0.0 : std::log2(static_cast<double>(theta));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool bf16 = flags & KF_PW_BF16;
-    if (neox) return bf16 ? qk_norm_rope_t<true, true>(p, s) : qk_norm_rope_t<false, true>(p, s);
-    return bf16 ? qk_norm_rope_t<true, false>(p, s) : qk_norm_rope_t<false, false>(p, s);
+    const unsigned grid = static_cast<unsigned>(blocks);
+    if (neox) return bf16 ? qk_norm_rope_t<true, true>(p, grid, s) : qk_norm_rope_t<false, true>(p, grid, s);
+    return bf16 ? qk_norm_rope_t<true, false>(p, grid, s) : qk_norm_rope_t<false, false>(p, grid, s);
 }
 
 int kf_swiglu(const void* gate_up, void* out, long long rows, int inter, unsigned flags, void* stream) {
@@ -1540,26 +1563,28 @@ int q4_attn_launch(const kf::Q4AttnParams& p, long long max_tiles, int sm_count,
 }
 
 int q4_io_params(const void* cache, const int* slots, const void* k, const void* v, int B, int S, int H_kv, int D,
-                 int n_blocks, int block_size, long long ksb, long long ksh, long long kss, long long vsb,
-                 long long vsh, long long vss, unsigned flags, kf::Q4IoParams* p) {
+                 int n_blocks, int block_size, const long long* strides, unsigned flags, kf::Q4IoParams* p) {
     if (flags & ~static_cast<unsigned>(KF_CACHE_BF16)) return KF_ERR_INVALID_ARG;
     if (B < 0 || S < 0 || H_kv <= 0 || H_kv > 65535 || n_blocks <= 0) return KF_ERR_INVALID_ARG;
     if (!q4_dim_ok(D)) return KF_ERR_UNSUPPORTED_HEAD_DIM;
     if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1))) return KF_ERR_INVALID_ARG;
-    drop_unused_strides(B, H_kv, S, ksb, ksh, kss);
-    drop_unused_strides(B, H_kv, S, vsb, vsh, vss);
-    if (!strides_ok(ksb, ksh, kss) || !strides_ok(vsb, vsh, vss)) return KF_ERR_INVALID_ARG;
+    if (!strides) return KF_ERR_INVALID_ARG;
+    long long st[6];
+    for (int i = 0; i < 6; ++i) st[i] = strides[i];
+    for (int i = 0; i < 6; i += 3) {
+        drop_unused_strides(B, H_kv, S, st[i], st[i + 1], st[i + 2]);
+        if (!strides_ok(st[i], st[i + 1], st[i + 2])) return KF_ERR_INVALID_ARG;
+    }
     if (static_cast<long long>(B) * S == 0) return KF_OK;
-    if (static_cast<long long>(B) * S > (1ll << 40)) return KF_ERR_INVALID_ARG;
     if (!cache || !slots || !k || !v) return KF_ERR_INVALID_ARG;
     if (!aligned16(cache) || !aligned16(k) || !aligned16(v)) return KF_ERR_MISALIGNED;
     p->cache = static_cast<uint8_t*>(const_cast<void*>(cache));
     p->slots = slots;
-    p->k = static_cast<uint16_t*>(const_cast<void*>(k));
-    p->v = static_cast<uint16_t*>(const_cast<void*>(v));
-    p->k_sb = ksb; p->k_sh = ksh; p->k_ss = kss;
-    p->v_sb = vsb; p->v_sh = vsh; p->v_ss = vss;
-    p->B = B;
+    p->k = static_cast<uint4*>(const_cast<void*>(k));
+    p->v = static_cast<uint4*>(const_cast<void*>(v));
+    p->k_sb = st[0] / 8; p->k_sh = st[1] / 8; p->k_ss = st[2] / 8;
+    p->v_sb = st[3] / 8; p->v_sh = st[4] / 8; p->v_ss = st[5] / 8;
+    p->n_tokens = static_cast<long long>(B) * S;
     p->S = S;
     p->H = H_kv;
     p->bs_log2 = log2_exact(block_size);
@@ -1568,12 +1593,15 @@ int q4_io_params(const void* cache, const int* slots, const void* k, const void*
 }
 
 template <int D, bool BF16>
-int q4_io_launch(const kf::Q4IoParams& p, bool write, cudaStream_t s) {
-    const long long blocks = (2ll * p.B * p.S * p.H + 7) / 8;
-    int grid = 0;
-    int rc = write ? pw_grid<kf::q4_write_kernel<D, BF16>>(256, blocks, &grid)
-                   : pw_grid<kf::q4_read_kernel<D, BF16>>(256, blocks, &grid);
+int q4_io_launch(kf::Q4IoParams p, bool write, cudaStream_t s) {
+    DeviceInfo* di = nullptr;
+    const int rc = device_info(&di);
     if (rc != KF_OK) return rc;
+    long long blocks = 0;
+    token_blocks(p.n_tokens, 2 * p.H, write ? 4096 / D : 2048 / D, kf::kQ4IoTokens, di->sm_count, &p.TPB, &p.splits,
+                 &p.rows_per_split, &blocks);
+    if (blocks >= (1ll << 31)) return KF_ERR_INVALID_ARG;
+    const unsigned grid = static_cast<unsigned>(blocks);
     if (write) kf::q4_write_kernel<D, BF16><<<grid, 256, 0, s>>>(p);
     else kf::q4_read_kernel<D, BF16><<<grid, 256, 0, s>>>(p);
     return launch_status();
@@ -1593,21 +1621,17 @@ int q4_io(const kf::Q4IoParams& p, int D, bool bf16, bool write, void* stream) {
 extern "C" {
 
 int kf_kv_write_q4(const void* k, const void* v, void* cache, const int* slots, int B, int S, int H_kv, int D,
-                   int n_blocks, int block_size, long long k_stride_b, long long k_stride_h, long long k_stride_s,
-                   long long v_stride_b, long long v_stride_h, long long v_stride_s, unsigned flags, void* stream) {
+                   int n_blocks, int block_size, const long long* strides, unsigned flags, void* stream) {
     kf::Q4IoParams p;
-    const int rc = q4_io_params(cache, slots, k, v, B, S, H_kv, D, n_blocks, block_size,
-                                k_stride_b, k_stride_h, k_stride_s, v_stride_b, v_stride_h, v_stride_s, flags, &p);
+    const int rc = q4_io_params(cache, slots, k, v, B, S, H_kv, D, n_blocks, block_size, strides, flags, &p);
     if (rc != KF_OK || static_cast<long long>(B) * S == 0) return rc;
     return q4_io(p, D, flags & KF_CACHE_BF16, true, stream);
 }
 
 int kf_kv_read_q4(const void* cache, const int* slots, void* k, void* v, int B, int S, int H_kv, int D, int n_blocks,
-                  int block_size, long long k_stride_b, long long k_stride_h, long long k_stride_s,
-                  long long v_stride_b, long long v_stride_h, long long v_stride_s, unsigned flags, void* stream) {
+                  int block_size, const long long* strides, unsigned flags, void* stream) {
     kf::Q4IoParams p;
-    const int rc = q4_io_params(cache, slots, k, v, B, S, H_kv, D, n_blocks, block_size,
-                                k_stride_b, k_stride_h, k_stride_s, v_stride_b, v_stride_h, v_stride_s, flags, &p);
+    const int rc = q4_io_params(cache, slots, k, v, B, S, H_kv, D, n_blocks, block_size, strides, flags, &p);
     if (rc != KF_OK || static_cast<long long>(B) * S == 0) return rc;
     return q4_io(p, D, flags & KF_CACHE_BF16, false, stream);
 }

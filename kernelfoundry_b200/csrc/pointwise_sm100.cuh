@@ -14,7 +14,9 @@
 // fp32 except the RoPE angle, which is formed and reduced modulo 2*pi in fp64
 // so that positions up to 2^31 keep the fp32 accuracy of sincosf.
 //
-// All three are HBM-streaming kernels: 16-byte vector loads and stores,
+// The query/key norm with the rotation (qk_norm_rope) rounds once, at the end.
+//
+// All are HBM-streaming kernels: 16-byte vector loads and stores,
 // inputs read once with the evict-first hint, grids sized from the occupancy
 // of the 148 SMs.  Nothing here is GEMM-shaped, so no tensor-core path.
 #pragma once
@@ -282,63 +284,170 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 }
 
 // ---- Query/key norm with RoPE ---------------------------------------------------
-// y = rnd(rot(x * rsqrt(mean(x^2) + eps) * w)) on every head row of Q and K: one warp per
-// row, the normalised row in shared memory between the norm and the rotation.
+// y = rnd(rot(x * rsqrt(mean(x^2) + eps) * w)) on every head row of Q and K.  Bound by HBM (each
+// element read once, written once); the rotation's angles are the same for all heads, so a block
+// takes whole tokens: it computes their cos / sin once into shared memory (angles reduced in
+// fp64, as rope_kernel) while its first rows are on their way.  A row belongs to GS = 2^k >= D / 16
+// threads with two 8-element vectors each, paired so that both halves of a NeoX rotation are in
+// one thread: vectors (u, u + rot_dim / 16) rotate, the rest pass through; the sum of squares is
+// reduced by shuffles.  Nothing but the angles goes through shared memory.
 struct QkNormRopeParams {
-    const uint16_t* q;
-    const uint16_t* k;
-    uint16_t* qo;
-    uint16_t* ko;
-    const uint16_t* qw;           // [D], nullptr: ones
-    const uint16_t* kw;
+    const uint4* q;
+    const uint4* k;
+    uint4* qo;
+    uint4* ko;
+    const uint4* qw;              // [D / 8], nullptr: ones
+    const uint4* kw;
     const int* pos;               // [B, S] positions, nullptr: position = s
     const float* inv_freq;        // [rot_dim / 2], nullptr: theta^(-2i/rot_dim)
-    long long q_sb, q_sh, q_ss, k_sb, k_sh, k_ss;        // element strides
+    long long q_sb, q_sh, q_ss, k_sb, k_sh, k_ss;        // strides in 16-byte vectors
     long long qo_sb, qo_sh, qo_ss, ko_sb, ko_sh, ko_ss;
     long long n_tokens;           // B * S
     int S, H_q, H_kv, D, rot_dim;
-    float eps, rot_scale;
+    int GS;                       // threads per row, a power of two
+    int TPB;                      // tokens per block
+    int splits, rows_per_split;   // blocks per token group and their rows (a multiple of 256 / GS)
+    float eps, rot_scale, inv_D;
     double log2_theta;
 };
 
+constexpr int kQkNormRopeTokens = 8;                       // the largest TPB
+
 template <bool BF16, bool NEOX>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormRopeParams p) {
-    __shared__ float s_row[8][512];
-    float* y = s_row[threadIdx.x >> 5];
-    const int lane = threadIdx.x & 31;
-    const int H = p.H_q + p.H_kv, half = p.rot_dim / 2;
-    for (long long r = (blockIdx.x * 256ll + threadIdx.x) >> 5; r < p.n_tokens * H; r += gridDim.x * 8ll) {
-        const long long t = r / H;
-        const int h = static_cast<int>(r % H);
-        const long long b = t / p.S, s = t % p.S;
-        const bool is_q = h < p.H_q;
-        const uint16_t* x = is_q ? p.q + b * p.q_sb + h * p.q_sh + s * p.q_ss
-                                 : p.k + b * p.k_sb + (h - p.H_q) * p.k_sh + s * p.k_ss;
-        uint16_t* o = is_q ? p.qo + b * p.qo_sb + h * p.qo_sh + s * p.qo_ss
-                           : p.ko + b * p.ko_sb + (h - p.H_q) * p.ko_sh + s * p.ko_ss;
-        const uint16_t* w = is_q ? p.qw : p.kw;
-        float ss = 0.f;
-        for (int d = lane; d < p.D; d += 32) {
-            y[d] = to_f32<BF16>(x[d]);
-            ss = fmaf(y[d], y[d], ss);
+    constexpr int UNR = 4;                                 // rows a thread has in flight
+    __shared__ double s_f[256];
+    __shared__ __align__(16) float s_cos[kQkNormRopeTokens * 256], s_sin[kQkNormRopeTokens * 256];
+    __shared__ long long s_off[4][kQkNormRopeTokens];      // q, k, q_out, k_out offsets of each token
+    __shared__ int s_pos[kQkNormRopeTokens];
+    const int tid = threadIdx.x, half = p.rot_dim >> 1, H = p.H_q + p.H_kv;
+    const int split = blockIdx.x % p.splits;
+    const long long tok0 = static_cast<long long>(blockIdx.x / p.splits) * p.TPB;
+    const int n_tok = p.n_tokens - tok0 < p.TPB ? static_cast<int>(p.n_tokens - tok0) : p.TPB;
+    if (tid < n_tok) {
+        const long long t = tok0 + tid, b = t / p.S, s = t - b * p.S;
+        s_off[0][tid] = b * p.q_sb + s * p.q_ss;
+        s_off[1][tid] = b * p.k_sb + s * p.k_ss;
+        s_off[2][tid] = b * p.qo_sb + s * p.qo_ss;
+        s_off[3][tid] = b * p.ko_sb + s * p.ko_ss;
+        s_pos[tid] = p.pos ? p.pos[t] : static_cast<int>(s);
+    }
+    for (int i = tid; i < half; i += 256)
+        s_f[i] = p.inv_freq ? static_cast<double>(p.inv_freq[i]) : exp2(-(2.0 * i / p.rot_dim) * p.log2_theta);
+    __syncthreads();
+
+    // row groups, this thread's, its place in the row, threads of a row that hold something
+    const int RG = 256 / p.GS, rg = tid / p.GS, u = tid & (p.GS - 1), U = p.D >> 4;
+    const int end = min((split + 1) * p.rows_per_split, n_tok * H);
+    int row = split * p.rows_per_split + rg;
+    int tk = row / H, h = row - tk * H;
+    // The thread's two vectors, and the first pair index of their rotation (-1: they pass through).
+    int c0, c1, p0 = -1, p1 = -1;
+    if (NEOX) {
+        const int r = p.rot_dim >> 4;
+        c0 = u < r ? u : 2 * u;
+        c1 = u < r ? u + r : 2 * u + 1;
+        if (u < r) p0 = 8 * u;
+    } else {
+        c0 = u;
+        c1 = u + U;
+        if (8 * c0 < p.rot_dim) p0 = 4 * c0;
+        if (8 * c1 < p.rot_dim) p1 = 4 * c1;
+    }
+    const bool on = u < U;
+    const uint4 one = pack8<BF16>({1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f});
+    uint4 w[2][2] = {{one, one}, {one, one}};
+    if (on && p.qw) { w[0][0] = __ldg(p.qw + c0); w[0][1] = __ldg(p.qw + c1); }
+    if (on && p.kw) { w[1][0] = __ldg(p.kw + c0); w[1][1] = __ldg(p.kw + c1); }
+
+    bool angles = false;
+    for (; row - rg < end; row += UNR * RG) {                            // (the same trips for the whole block)
+        uint4 v[UNR][2];
+        uint4* out[UNR];
+        int at[UNR];                                                     // token, or -1: no row
+        bool is_q[UNR];
+#pragma unroll
+        for (int i = 0; i < UNR; ++i) {
+            at[i] = -1;
+            v[i][0] = v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (row + i * RG < end) {
+                at[i] = tk;
+                is_q[i] = h < p.H_q;
+                const uint4* src = is_q[i] ? p.q + s_off[0][tk] + h * p.q_sh : p.k + s_off[1][tk] + (h - p.H_q) * p.k_sh;
+                out[i] = is_q[i] ? p.qo + s_off[2][tk] + h * p.qo_sh : p.ko + s_off[3][tk] + (h - p.H_q) * p.ko_sh;
+                if (on) {
+                    v[i][0] = ld_stream(src + c0);
+                    v[i][1] = ld_stream(src + c1);
+                }
+            }
+            for (h += RG; h >= H; h -= H) ++tk;
         }
-        for (int m = 16; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-        const float rinv = rsqrtf(ss / p.D + p.eps);
-        for (int d = lane; d < p.D; d += 32) y[d] *= rinv * (w ? to_f32<BF16>(w[d]) : 1.f);
-        __syncwarp();
-        const int pos = p.pos ? p.pos[t] : static_cast<int>(s);
-        for (int i = lane; i < half; i += 32) {
-            const double f = p.inv_freq ? static_cast<double>(p.inv_freq[i]) : exp2(-(2.0 * i / p.rot_dim) * p.log2_theta);
-            float sn, cs;
-            sincosf(reduce_2pi(pos * f), &sn, &cs);
-            sn *= p.rot_scale;
-            cs *= p.rot_scale;
-            const int i0 = NEOX ? i : 2 * i, i1 = NEOX ? i + half : 2 * i + 1;
-            o[i0] = from_f32<BF16>(fmaf(y[i0], cs, -y[i1] * sn));
-            o[i1] = from_f32<BF16>(fmaf(y[i1], cs, y[i0] * sn));
+        if (!angles) {                                                   // while the first rows are on their way
+            for (int i = tid; i < n_tok * half; i += 256) {
+                const int t = i / half;
+                float sn, cs;
+                sincosf(reduce_2pi(s_pos[t] * s_f[i - t * half]), &sn, &cs);
+                s_cos[i] = cs * p.rot_scale;
+                s_sin[i] = sn * p.rot_scale;
+            }
+            __syncthreads();
+            angles = true;
         }
-        for (int d = p.rot_dim + lane; d < p.D; d += 32) o[d] = from_f32<BF16>(y[d]);
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < UNR; ++i) {
+            float x[2][8], ss = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                unpack8<BF16>(v[i][c], x[c]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss = fmaf(x[c][e], x[c][e], ss);
+            }
+            for (int o = p.GS >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (at[i] < 0 || !on) continue;
+            const float r = rsqrtf(fmaf(ss, p.inv_D, p.eps));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float wt[8];
+                unpack8<BF16>(is_q[i] ? w[0][c] : w[1][c], wt);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][e] *= r * wt[e];
+            }
+            const float* cs = s_cos + at[i] * half;
+            const float* sn = s_sin + at[i] * half;
+            if (NEOX) {
+                if (p0 >= 0) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const float4 c4 = *reinterpret_cast<const float4*>(cs + p0 + 4 * g);
+                        const float4 s4 = *reinterpret_cast<const float4*>(sn + p0 + 4 * g);
+                        const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, sc[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float a = x[0][4 * g + e], b = x[1][4 * g + e];
+                            x[0][4 * g + e] = fmaf(a, cc[e], -b * sc[e]);
+                            x[1][4 * g + e] = fmaf(b, cc[e], a * sc[e]);
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int pr = c ? p1 : p0;
+                    if (pr < 0) continue;
+                    const float4 c4 = *reinterpret_cast<const float4*>(cs + pr);
+                    const float4 s4 = *reinterpret_cast<const float4*>(sn + pr);
+                    const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, sc[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = x[c][2 * e], b = x[c][2 * e + 1];
+                        x[c][2 * e] = fmaf(a, cc[e], -b * sc[e]);
+                        x[c][2 * e + 1] = fmaf(b, cc[e], a * sc[e]);
+                    }
+                }
+            }
+            st_stream(out[i] + c0, pack8<BF16>(x[0]));
+            st_stream(out[i] + c1, pack8<BF16>(x[1]));
+        }
     }
 }
 

@@ -14,8 +14,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import (KF_CACHE_BF16, KF_FLAG_CAUSAL, KF_FLAG_OUT_BF16, KF_FLAG_OUT_F16, KF_FLAG_Q_BF16, lib,
-                   on_device)
+from ._lib import (KF_CACHE_BF16, KF_FLAG_CAUSAL, KF_FLAG_OUT_BF16, KF_FLAG_OUT_F16, KF_FLAG_Q_BF16,
+                   CallPlans, lib, on_device, strides_arg)
 
 __all__ = ["q4_cache", "kv_write_q4", "kv_read_q4", "flash_attn_paged_q4"]
 
@@ -82,6 +82,19 @@ def kv_write_q4(k, v, cache, slots, *, layout: str = "bhsd") -> None:
     strides (multiples of 8) with a contiguous head dimension.  slots: int32 ``[B, S]``; slot
     t is row ``t % block_size`` of block ``t // block_size``; one outside the cache (-1) is
     skipped.  Each head row is quantised by itself (scale and zero point per row)."""
+    key = (layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, cache.shape,
+           cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
+    plan = _write_plans.get(key) or _write_plans.put(key, _plan_io(cache, slots, k, v, layout))
+    index, dims, (_, strides), flags = plan
+    on_device(index, lib().kf_kv_write_q4, "kf_kv_write_q4", k.data_ptr(), v.data_ptr(), cache.data_ptr(),
+              slots.data_ptr(), *dims, strides, flags)
+
+
+_write_plans, _read_plans, _attn_plans = CallPlans(), CallPlans(), CallPlans()
+
+
+def _plan_io(cache, slots, k, v, layout):
+    """Checks of a write or read and the arguments that follow from its tensors' form."""
     n_blocks, H_kv, bs, D = _cache_dims(cache)
     dev = cache.device
     (B, H, S, Dk), ks = _tokens(k, "k", layout, dev)
@@ -91,8 +104,7 @@ def kv_write_q4(k, v, cache, slots, *, layout: str = "bhsd") -> None:
     if (H, Dk) != (H_kv, D):
         raise ValueError(f"k and v must have the cache's {H_kv} heads of {D}")
     _check_slots(slots, B, S, dev)
-    on_device(dev.index, lib().kf_kv_write_q4, "kf_kv_write_q4", k.data_ptr(), v.data_ptr(), cache.data_ptr(),
-              slots.data_ptr(), B, S, H, D, n_blocks, bs, *ks, *vs, _IO_FLAGS[k.dtype])
+    return dev.index, (B, S, H, D, n_blocks, bs), strides_arg(*ks, *vs), _IO_FLAGS[k.dtype]
 
 
 def kv_read_q4(cache, slots, *, dtype=torch.float16, layout: str = "bhsd", out=None):
@@ -100,24 +112,20 @@ def kv_read_q4(cache, slots, *, dtype=torch.float16, layout: str = "bhsd", out=N
 
     ``[B, H_kv, S, D]`` ("bhsd", what :func:`flash_attn_fwd` takes) or ``[B, S, H_kv, D]``
     ("bshd").  A slot outside the cache reads zeros.  ``out``: (k, v) to write into."""
-    n_blocks, H_kv, bs, D = _cache_dims(cache)
-    dev = cache.device
-    if slots.dim() != 2:
-        raise ValueError("slots must be a contiguous int32 [B, S] tensor")
-    B, S = slots.shape
-    _check_slots(slots, B, S, dev)
     if out is None:
-        if layout not in ("bhsd", "bshd") or dtype not in _IO_FLAGS:
-            raise ValueError("layout must be 'bhsd' or 'bshd' and dtype float16 or bfloat16")
+        _, H_kv, _, D = _cache_dims(cache)
+        if slots.dim() != 2 or layout not in ("bhsd", "bshd") or dtype not in _IO_FLAGS:
+            raise ValueError("slots must be [B, S], layout 'bhsd' or 'bshd', dtype float16 or bfloat16")
+        B, S = slots.shape
         shape = (B, H_kv, S, D) if layout == "bhsd" else (B, S, H_kv, D)
-        out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+        out = (torch.empty(shape, dtype=dtype, device=cache.device), torch.empty(shape, dtype=dtype, device=cache.device))
     k, v = out
-    dims_k, ks = _tokens(k, "out k", layout, dev)
-    dims_v, vs = _tokens(v, "out v", layout, dev)
-    if dims_k != (B, H_kv, S, D) or dims_v != dims_k or k.dtype != v.dtype:
-        raise ValueError(f"out must be two tensors of B={B}, H={H_kv}, S={S}, D={D} and one type")
-    on_device(dev.index, lib().kf_kv_read_q4, "kf_kv_read_q4", cache.data_ptr(), slots.data_ptr(), k.data_ptr(),
-            v.data_ptr(), B, S, H_kv, D, n_blocks, bs, *ks, *vs, _IO_FLAGS[k.dtype])
+    key = (layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, cache.shape,
+           cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
+    plan = _read_plans.get(key) or _read_plans.put(key, _plan_io(cache, slots, k, v, layout))
+    index, dims, (_, strides), flags = plan
+    on_device(index, lib().kf_kv_read_q4, "kf_kv_read_q4", cache.data_ptr(), slots.data_ptr(), k.data_ptr(),
+              v.data_ptr(), *dims, strides, flags)
     return k, v
 
 
@@ -133,6 +141,30 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
     with ``return_lse`` also (Mi, Li), the row max of the scaled scores and sum of exp(s - Mi).
     Each stream has its workspace; ``workspace`` (zero-filled uint8,
     ``kf_attn_paged_q4_workspace_bytes``) replaces it, e.g. for a captured graph."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("out and out_dtype disagree")
+    key = (causal, q.shape, q.stride(), q.dtype, q.device, cache.shape, cache.stride(), cache.dtype, cache.device,
+           block_table.shape, block_table.stride(), block_table.dtype, block_table.device, seq_lens.shape,
+           seq_lens.stride(), seq_lens.dtype, seq_lens.device, out.shape, out.stride(), out.dtype, out.device)
+    plan = _attn_plans.get(key) or _attn_plans.put(key, _plan_attn(q, cache, block_table, seq_lens, out, causal))
+    device, dims, flags, need = plan
+    if workspace is None:
+        workspace = _workspace(device, need)
+    Mi = Li = None
+    if return_lse:
+        Mi = torch.empty(q.shape[:3], dtype=torch.float32, device=device)
+        Li = torch.empty_like(Mi)
+    on_device(device.index, lib().kf_attn_fwd_paged_q4, "kf_attn_fwd_paged_q4", q.data_ptr(), cache.data_ptr(),
+              block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), Mi.data_ptr() if return_lse else None,
+              Li.data_ptr() if return_lse else None, *dims, 0.0 if scale is None else scale, flags,
+              workspace.data_ptr(), workspace.numel())
+    return (out, Mi, Li) if return_lse else out
+
+
+def _plan_attn(q, cache, block_table, seq_lens, out, causal):
+    """Checks of :func:`flash_attn_paged_q4` and the arguments that follow from its tensors' form."""
     n_blocks, H_kv, bs, D = _cache_dims(cache)
     dev = cache.device
     if q.dtype not in _IO_FLAGS or q.dim() != 4 or not q.is_contiguous() or q.device != dev or q.shape[3] != D:
@@ -141,26 +173,12 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
     for t, name, nd in ((block_table, "block_table", 2), (seq_lens, "seq_lens", 1)):
         if t.dtype != torch.int32 or t.dim() != nd or t.shape[0] != B or t.device != dev or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {nd}-D int32 tensor with {B} rows on {dev}")
-    max_blocks = block_table.shape[1]
-    if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise ValueError("out and out_dtype disagree")
     if out.dtype not in _OUT_FLAGS:
         raise ValueError("output dtype must be float32, float16 or bfloat16")
     if out.shape != q.shape or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be a contiguous {tuple(q.shape)} tensor on {dev}")
-    Mi = Li = None
-    if return_lse:
-        Mi = torch.empty((B, H_q, S_q), dtype=torch.float32, device=dev)
-        Li = torch.empty_like(Mi)
+    max_blocks = block_table.shape[1]
     flags = (KF_FLAG_CAUSAL if causal else 0) | _OUT_FLAGS[out.dtype] | (KF_FLAG_Q_BF16 if q.dtype == torch.bfloat16 else 0)
-    L = lib()
-    if workspace is None:
-        workspace = _workspace(dev, L.kf_attn_paged_q4_workspace_bytes(B, H_q, H_kv, S_q, D, bs, max_blocks))
-    on_device(dev.index, L.kf_attn_fwd_paged_q4, "kf_attn_fwd_paged_q4", q.data_ptr(), cache.data_ptr(),
-            block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), Mi.data_ptr() if return_lse else None,
-            Li.data_ptr() if return_lse else None, B, H_q, H_kv, S_q, D, n_blocks, bs, max_blocks,
-            0.0 if scale is None else float(scale), flags, workspace.data_ptr() if workspace is not None else None,
-            workspace.numel() if workspace is not None else 0)
-    return (out, Mi, Li) if return_lse else out
+    with torch.cuda.device(dev):
+        need = lib().kf_attn_paged_q4_workspace_bytes(B, H_q, H_kv, S_q, D, bs, max_blocks)
+    return dev, (B, H_q, H_kv, S_q, D, n_blocks, bs, max_blocks), flags, max(need, 16)

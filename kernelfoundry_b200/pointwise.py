@@ -12,7 +12,7 @@ import ctypes
 
 import torch
 
-from ._lib import KF_PW_BF16, KF_ROPE_GPTJ, check, lib, on_device
+from ._lib import KF_PW_BF16, KF_ROPE_GPTJ, CallPlans, check, lib, on_device, strides_arg
 
 __all__ = ["rms_norm", "fused_add_rms_norm", "rope_", "qk_norm_rope", "swiglu"]
 
@@ -143,24 +143,43 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     ``out``: ``(q_out, k_out)`` in ``layout`` to write into -- q and k themselves for in place,
     or e.g. transposed views to change the storage order.
     """
+    if out is None:
+        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+               torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None)
+    q_out, k_out = out
+    key = (layout, interleaved, rot_dim, *(None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+                                           for t in (q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq)))
+    plan = _qk_plans.get(key) or _qk_plans.put(key, _plan_qk_norm_rope(
+        q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq, layout, interleaved, rot_dim))
+    index, (B, S, H_q, H_kv, D, rot), (_, strides), flags = plan
+    on_device(index, lib().kf_qk_norm_rope, "kf_qk_norm_rope", q.data_ptr(), k.data_ptr() if k is not None else None,
+              q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
+              q_out.data_ptr(), k_out.data_ptr() if k_out is not None else None,
+              positions.data_ptr() if positions is not None else None, inv_freq.data_ptr() if inv_freq is not None else None,
+              B, S, H_q, H_kv, D, rot, theta, rot_scale, eps, strides, flags)
+    return q_out, k_out
+
+
+_qk_plans = CallPlans()
+
+
+def _plan_qk_norm_rope(q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq, layout, interleaved, rot_dim):
+    """Checks of :func:`qk_norm_rope` and the arguments that follow from its tensors' form."""
     dev, D = q.device, q.shape[-1]
     if layout not in ("bhsd", "bshd"):
         raise ValueError("layout must be 'bhsd' or 'bshd'")
-    if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=dev),
-               torch.empty(k.shape, dtype=k.dtype, device=dev) if k is not None else None)
-    q_out, k_out = out
     flag = _DT_FLAGS.get(q.dtype)
     if flag is None or not q.is_cuda:
         raise ValueError("tensors must be float16 or bfloat16 CUDA tensors (no CPU path)")
     s, h = (2, 1) if layout == "bhsd" else (1, 2)
-    strides, heads = [], []
+    strides, heads = [[], []], []
     for x, y in ((q, q_out), (k, k_out)):
         if x is None:
             if y is not None:
                 raise ValueError("k_out without k")
             heads.append(0)
-            strides += [0] * 6
+            strides[0] += [0, 0, 0]
+            strides[1] += [0, 0, 0]
             continue
         for t in (x, y):
             if t is None or t.dtype != q.dtype or t.device != dev or t.dim() != 4 or t.stride(3) != 1:
@@ -168,9 +187,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
         if y.shape != x.shape or x.shape[0] != q.shape[0] or x.shape[s] != q.shape[s] or x.shape[3] != D:
             raise ValueError("k must match q in B, S and D, and out q and k")
         heads.append(x.shape[h])
-        for t in (x, y):
+        for t, to in ((x, strides[0]), (y, strides[1])):
             st = t.stride()
-            strides += [st[0], st[h], st[s]]
+            to += [st[0], st[h], st[s]]
     B, S = q.shape[0], q.shape[s]
     for w in (q_weight, k_weight):
         if w is not None and (w.dtype != q.dtype or w.device != dev or w.dim() != 1 or w.shape[0] != D
@@ -183,15 +202,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2
                                  or not inv_freq.is_contiguous() or inv_freq.device != dev):
         raise ValueError("inv_freq must be a contiguous float32 [rot_dim/2] tensor on q's device")
-    qi, qo, ki, ko = strides[0:3], strides[3:6], strides[6:9], strides[9:12]
-
-    def ptr(t):
-        return t.data_ptr() if t is not None else None
-
-    on_device(dev.index, lib().kf_qk_norm_rope, "kf_qk_norm_rope", q.data_ptr(), ptr(k), ptr(q_weight), ptr(k_weight),
-              q_out.data_ptr(), ptr(k_out), ptr(positions), ptr(inv_freq), B, S, heads[0], heads[1], D, rot,
-              theta, rot_scale, eps, *qi, *ki, *qo, *ko, flag | (KF_ROPE_GPTJ if interleaved else 0))
-    return q_out, k_out
+    return (dev.index, (B, S, heads[0], heads[1], D, rot), strides_arg(*strides[0], *strides[1]),
+            flag | (KF_ROPE_GPTJ if interleaved else 0))
 
 
 def swiglu(gate_up: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -23,8 +23,12 @@ def test_cache_header_symbols(kf_lib):
         assert hasattr(kf_lib, s)
 
 
+def _strides(*st):
+    return (ctypes.c_longlong * len(st))(*st)
+
+
 def _io(fn, a=FAKE, b=FAKE, c=FAKE, d=FAKE, B=1, S=4, H=2, D=128, nb=4, bs=16, st=(1024, 512, 128), vst=None, flags=0):
-    return fn(a, b, c, d, B, S, H, D, nb, bs, *st, *(vst or st), flags, None)
+    return fn(a, b, c, d, B, S, H, D, nb, bs, _strides(*st, *(vst or st)), flags, None)
 
 
 def test_write_and_read_arguments(kf_lib):
@@ -60,8 +64,8 @@ def test_qk_norm_rope_arguments(kf_lib):
 
     def call(q=FAKE, k=FAKE, qw=None, qo_=FAKE, ko_=FAKE, B=2, S=4, Hq=4, Hkv=2, D=128, rot=128, theta=1e4, sc=1.0, eps=1e-6,
              st=(2048, 512, 128), flags=0):
-        return kf_lib.kf_qk_norm_rope(q, k, qw, None, qo_, ko_, None, None, B, S, Hq, Hkv, D, rot, theta, sc, eps, *st, *st, *st,
-                                      *st, flags, None)
+        return kf_lib.kf_qk_norm_rope(q, k, qw, None, qo_, ko_, None, None, B, S, Hq, Hkv, D, rot, theta, sc, eps,
+                                      _strides(*st, *st, *st, *st), flags, None)
 
     for kw in (dict(D=24), dict(D=528), dict(rot=8), dict(rot=144), dict(rot=-16), dict(theta=0.0), dict(eps=-1.0),
                dict(sc=float("nan")), dict(flags=4), dict(q=None), dict(ko_=None), dict(Hq=0, Hkv=0), dict(B=-1),
