@@ -113,20 +113,36 @@ def kv_read_q4(cache, slots, *, dtype=torch.float16, layout: str = "bhsd", out=N
     ``[B, H_kv, S, D]`` ("bhsd", what :func:`flash_attn_fwd` takes) or ``[B, S, H_kv, D]``
     ("bshd").  A slot outside the cache reads zeros.  ``out``: (k, v) to write into."""
     if out is None:
-        _, H_kv, _, D = _cache_dims(cache)
-        if slots.dim() != 2 or layout not in ("bhsd", "bshd") or dtype not in _IO_FLAGS:
-            raise ValueError("slots must be [B, S], layout 'bhsd' or 'bshd', dtype float16 or bfloat16")
-        B, S = slots.shape
-        shape = (B, H_kv, S, D) if layout == "bhsd" else (B, S, H_kv, D)
-        out = (torch.empty(shape, dtype=dtype, device=cache.device), torch.empty(shape, dtype=dtype, device=cache.device))
-    k, v = out
-    key = (layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, cache.shape,
-           cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
-    plan = _read_plans.get(key) or _read_plans.put(key, _plan_io(cache, slots, k, v, layout))
-    index, dims, (_, strides), flags = plan
+        key = (layout, dtype, cache.shape, cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(),
+               slots.dtype, slots.device)
+        plan = _read_plans.get(key) or _read_plans.put(key, _plan_read(cache, slots, dtype, layout))
+        shape, device, (index, dims, (_, strides), flags) = plan
+        k = torch.empty(shape, dtype=dtype, device=device)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        key = (layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, cache.shape,
+               cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
+        plan = _read_plans.get(key) or _read_plans.put(key, _plan_io(cache, slots, k, v, layout))
+        index, dims, (_, strides), flags = plan
     on_device(index, lib().kf_kv_read_q4, "kf_kv_read_q4", cache.data_ptr(), slots.data_ptr(), k.data_ptr(),
               v.data_ptr(), *dims, strides, flags)
     return k, v
+
+
+def _plan_read(cache, slots, dtype, layout):
+    """Shape of a read's results and the plan of reading into such tensors."""
+    n_blocks, H_kv, bs, D = _cache_dims(cache)
+    if slots.dim() != 2 or layout not in ("bhsd", "bshd") or dtype not in _IO_FLAGS:
+        raise ValueError("slots must be [B, S], layout 'bhsd' or 'bshd', dtype float16 or bfloat16")
+    B, S = slots.shape
+    _check_slots(slots, B, S, cache.device)
+    if layout == "bhsd":
+        shape, strides = (B, H_kv, S, D), (H_kv * S * D, S * D, D)
+    else:
+        shape, strides = (B, S, H_kv, D), (H_kv * S * D, D, H_kv * D)
+    return shape, cache.device, (cache.device.index, (B, S, H_kv, D, n_blocks, bs), strides_arg(*strides, *strides),
+                                 _IO_FLAGS[dtype])
 
 
 def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=None, out=None, out_dtype=None,
@@ -142,7 +158,7 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
     Each stream has its workspace; ``workspace`` (zero-filled uint8,
     ``kf_attn_paged_q4_workspace_bytes``) replaces it, e.g. for a captured graph."""
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
+        out = torch.empty_like(q, dtype=out_dtype) if out_dtype is not None else torch.empty_like(q)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise ValueError("out and out_dtype disagree")
     key = (causal, q.shape, q.stride(), q.dtype, q.device, cache.shape, cache.stride(), cache.dtype, cache.device,

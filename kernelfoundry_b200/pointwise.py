@@ -144,8 +144,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     or e.g. transposed views to change the storage order.
     """
     if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-               torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None)
+        out = (torch.empty_like(q, memory_format=torch.contiguous_format),
+               torch.empty_like(k, memory_format=torch.contiguous_format) if k is not None else None)
     q_out, k_out = out
     key = (layout, interleaved, rot_dim, *(None if t is None else (t.shape, t.stride(), t.dtype, t.device)
                                            for t in (q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq)))
