@@ -48,13 +48,18 @@ __device__ __forceinline__ uint32_t q4_codes8(const float (&x)[8], float inv, fl
     const float m = 12582912.0f, lo = m - zp, hi = lo + 15.0f;
     float n[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        n[e] = __fadd_rn(fminf(fmaxf(__fadd_rn(__fmul_rn(x[e], inv), m), lo), hi), -lo);
+    for (int e = 0; e < 8; e += 2) {
+        // (not packed: a packed product and sum of explicit rounding were still fused into one FMA)
+        const float q0 = __fadd_rn(__fmul_rn(x[e], inv), m), q1 = __fadd_rn(__fmul_rn(x[e + 1], inv), m);
+        const float2 y = fadd2(make_float2(fminf(fmaxf(q0, lo), hi), fminf(fmaxf(q1, lo), hi)), make_float2(-lo, -lo));
+        n[e] = y.x;
+        n[e + 1] = y.y;
+    }
     float h[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         h[i] = fmaf(fmaf(n[4 * i + 3], 16.0f, n[4 * i + 2]), 256.0f, fmaf(n[4 * i + 1], 16.0f, n[4 * i]));
-    return static_cast<uint32_t>(h[0]) | static_cast<uint32_t>(h[1]) << 16;
+    return __float2uint_rz(h[0]) | __float2uint_rz(h[1]) << 16;
 }
 
 __device__ __forceinline__ float fmax_nan(float a, float b) {
@@ -111,7 +116,7 @@ __device__ __forceinline__ int q4_tokens(const Q4IoParams& p, Q4Tokens& tok, lon
 // A row belongs to D / 16 threads with the vectors u and u + D / 16: a store of their words is a
 // whole sector.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) q4_write_kernel(const Q4IoParams p) {
+__global__ void __launch_bounds__(256, 3) q4_write_kernel(const Q4IoParams p) {
     constexpr int GS = D / 16, RG = 256 / GS, UNR = 4;
     __shared__ Q4Tokens tok;
     const int tid = threadIdx.x, u = tid % GS, H2 = 2 * p.H, split = blockIdx.x % p.splits;
@@ -174,10 +179,31 @@ __global__ void __launch_bounds__(256) q4_write_kernel(const Q4IoParams p) {
     }
 }
 
-// A row belongs to D / 8 threads with a word (8 codes, one 16-byte vector) each.
+// Eight values s * (n - z) of a word.  A nibble in place, at bit 4e, under the exponent of 2^23 is
+// 2^23 + n 16^e; taking away 2^23 + z 16^e is exact, and s 16^-e puts the product back (exact
+// powers of two, so each value is rounded once, as s * (n - z) is).  Nibbles 5..7 come from the
+// word shifted by 20.  zc, sc: {2^23 + z 16^e}, {s 16^-e} for e = 0..4.
+__device__ __forceinline__ void q4_values8(uint32_t w, const float (&zc)[5], const float (&sc)[5], float (&x)[8]) {
+    const uint32_t v = w >> 20;
+    float n[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int at = e < 5 ? e : e - 5;
+        n[e] = __uint_as_float(((e < 5 ? w : v) & (15u << (4 * at))) | 0x4B000000u);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const int a = e < 5 ? e : e - 5, b = e + 1 < 5 ? e + 1 : e + 1 - 5;
+        const float2 y = fmul2(fadd2(make_float2(n[e], n[e + 1]), make_float2(-zc[a], -zc[b])), make_float2(sc[a], sc[b]));
+        x[e] = y.x;
+        x[e + 1] = y.y;
+    }
+}
+
+// A row belongs to D / 16 threads with the words (8 codes, one 16-byte vector) u and u + D / 16.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) q4_read_kernel(const Q4IoParams p) {
-    constexpr int GS = D / 8, RG = 256 / GS, UNR = 8;
+__global__ void __launch_bounds__(256, 4) q4_read_kernel(const Q4IoParams p) {
+    constexpr int GS = D / 16, RG = 256 / GS, UNR = 4;
     __shared__ Q4Tokens tok;
     const int tid = threadIdx.x, u = tid % GS, H2 = 2 * p.H, split = blockIdx.x % p.splits;
     const int n = q4_tokens<D>(p, tok, static_cast<long long>(blockIdx.x / p.splits) * p.TPB);
@@ -186,12 +212,12 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4IoParams p) {
     int row = split * p.rows_per_split + tid / GS;
     int t = row / H2, r = row - t * H2;
     for (; row < end; row += UNR * RG) {
-        uint32_t w[UNR], word[UNR];
+        uint32_t w[UNR][2], word[UNR];
         uint4* dst[UNR];
 #pragma unroll
         for (int i = 0; i < UNR; ++i) {
             dst[i] = nullptr;
-            w[i] = word[i] = 0u;
+            w[i][0] = w[i][1] = word[i] = 0u;
             if (row + i * RG < end) {
                 const bool is_v = r >= p.H;
                 const int h = is_v ? r - p.H : r;
@@ -199,7 +225,9 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4IoParams p) {
                 if (tok.group[t] >= 0) {
                     const uint8_t* g = p.cache + tok.group[t] + h * head;
                     const int rr = tok.row[t];
-                    w[i] = __ldg(reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW) + u);
+                    const uint32_t* c = reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW) + u;
+                    w[i][0] = __ldg(c);
+                    w[i][1] = __ldg(c + GS);
                     word[i] = __ldg(reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS)) + rr);
                 }
             }
@@ -208,12 +236,19 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const Q4IoParams p) {
 #pragma unroll
         for (int i = 0; i < UNR; ++i) {
             if (!dst[i]) continue;
-            const float s = q4_scale(word[i]), z = __uint_as_float(0x4B000000u | (word[i] & 15u));
-            float x[8];
+            const float s = q4_scale(word[i]), z = __uint_as_float(0x4B000000u | (word[i] & 15u)) - 8388608.0f;
+            float zc[5], sc[5];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[e] = s * (__uint_as_float(0x4B000000u | ((w[i] >> (4 * e)) & 15u)) - z);   // 2^23 + n, 2^23 + z: exact
-            st_stream(dst[i], pack8<BF16>(x));
+            for (int e = 0; e < 5; ++e) {
+                zc[e] = fmaf(z, static_cast<float>(1 << (4 * e)), 8388608.0f);
+                sc[e] = s * (1.0f / static_cast<float>(1 << (4 * e)));
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float x[8];
+                q4_values8(w[i][c], zc, sc, x);
+                st_stream(dst[i] + c * GS, pack8<BF16>(x));
+            }
         }
     }
 }

@@ -128,14 +128,6 @@ struct Q4Warp {                    // a warp's running state of one unit; pairs:
     float tlim, tnorm, tinv;       // value scales up to tlim times tnorm stay below 2^7; tinv = 1 / tnorm
 };
 
-__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
-        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 __device__ __forceinline__ float2 fmax2(float2 a, float2 b) { return make_float2(fmaxf(a.x, b.x), fmaxf(a.y, b.y)); }
 
 __device__ __forceinline__ int q4_len(const Q4AttnParams& p, int b) {

@@ -1340,13 +1340,15 @@ int qk_norm_rope_t(const kf::QkNormRopeParams& p, unsigned grid, cudaStream_t s)
     return launch_status();
 }
 
+const int kTokenBlockWaves = std::getenv("KF_TBW") ? std::atoi(std::getenv("KF_TBW")) : 2;
+
 // Blocks of `per` tokens with `rows` rows each (a block passes over `group` rows at a time): as
-// many tokens as leave two blocks an SM, and where even single tokens are fewer than that, the
-// rows of a token are split.
-void token_blocks(long long n_tokens, int rows, int group, int max_per, int sm_count, int* per, int* splits,
+// many tokens as leave `waves` blocks an SM, and where even single tokens are fewer than two blocks
+// an SM, the rows of a token are split.
+void token_blocks(long long n_tokens, int rows, int group, int max_per, int waves, int sm_count, int* per, int* splits,
                   int* rows_per_split, long long* blocks) {
     int t = max_per;
-    while (t > 1 && (n_tokens + t - 1) / t < 2ll * sm_count) t >>= 1;
+    while (t > 1 && (n_tokens + t - 1) / t < static_cast<long long>(waves) * sm_count) t >>= 1;
     *per = t;
     const int passes = (t * rows + group - 1) / group;
     long long sp = t > 1 ? 1 : 2ll * sm_count / (n_tokens > 0 ? n_tokens : 1);
@@ -1433,7 +1435,7 @@ int kf_rope(void* q, void* k, const int* positions, const float* inv_freq, int B
     int hg_target = 64 / p.U;
     if (hg_target < 1) hg_target = 1;
     const int need = (H + hg_target - 1) / hg_target;
-    const int hb = need <= 1 ? 1 : need <= 4 ? 4 : 8;
+    const int hb = need <= 1 ? 1 : need <= 4 ? 4 : 2;
     p.HG = (H + hb - 1) / hb;
     p.TPB = 256 / (p.U * p.HG);
     if (p.TPB < 1) p.TPB = 1;
@@ -1494,7 +1496,9 @@ int kf_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
     p.GS = 1;
     while (p.GS < D / 16) p.GS <<= 1;
     long long blocks = 0;
-    token_blocks(n_tokens, H_q + H_kv, 256 / p.GS, kf::kQkNormRopeTokens, di->sm_count, &p.TPB, &p.splits,
+    int most = kf::kQkNormRopeTokens;
+    while (most * (D / 2) > kf::kQkNormRopePairs) most >>= 1;
+    token_blocks(n_tokens, H_q + H_kv, 256 / p.GS, most, kTokenBlockWaves, di->sm_count, &p.TPB, &p.splits,
                  &p.rows_per_split, &blocks);
     if (blocks >= (1ll << 31)) return KF_ERR_INVALID_ARG;
     p.eps = eps;
@@ -1598,7 +1602,7 @@ int q4_io_launch(kf::Q4IoParams p, bool write, cudaStream_t s) {
     const int rc = device_info(&di);
     if (rc != KF_OK) return rc;
     long long blocks = 0;
-    token_blocks(p.n_tokens, 2 * p.H, write ? 4096 / D : 2048 / D, kf::kQ4IoTokens, di->sm_count, &p.TPB, &p.splits,
+    token_blocks(p.n_tokens, 2 * p.H, 4096 / D, kf::kQ4IoTokens, kTokenBlockWaves, di->sm_count, &p.TPB, &p.splits,
                  &p.rows_per_split, &blocks);
     if (blocks >= (1ll << 31)) return KF_ERR_INVALID_ARG;
     const unsigned grid = static_cast<unsigned>(blocks);

@@ -438,7 +438,7 @@ __device__ __forceinline__ float fmax3f(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// Packed fp32 pairs (one instruction each on sm_100): d = a * b + c, d = a + b.
+// Packed fp32 pairs (one instruction each on sm_100): d = a * b + c, d = a + b, d = a * b.
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
     float2 d;
     asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
@@ -456,6 +456,14 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 // 2^x on the FMA pipe, two lanes per instruction, for x in [-125, 8] (softmax exponents:
 // scores minus a reference max): round-to-nearest split x = j + f, f in [-0.5, 0.5], with the
 // 1.5 * 2^23 shift; 2^f by a degree-3 polynomial least-squares fitted for relative error

@@ -25,6 +25,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "kf_ptx.cuh"
+
 namespace kf {
 
 // ---- 8 x 16-bit <-> 8 x fp32 -------------------------------------------------
@@ -286,11 +288,14 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 // ---- Query/key norm with RoPE ---------------------------------------------------
 // y = rnd(rot(x * rsqrt(mean(x^2) + eps) * w)) on every head row of Q and K.  Bound by HBM (each
 // element read once, written once); the rotation's angles are the same for all heads, so a block
-// takes whole tokens: it computes their cos / sin once into shared memory (angles reduced in
-// fp64, as rope_kernel) while its first rows are on their way.  A row belongs to GS = 2^k >= D / 16
-// threads with two 8-element vectors each, paired so that both halves of a NeoX rotation are in
-// one thread: vectors (u, u + rot_dim / 16) rotate, the rest pass through; the sum of squares is
-// reduced by shuffles.  Nothing but the angles goes through shared memory.
+// takes whole tokens: while its first rows are on their way it computes each pair's four
+// coefficients (cos and sin times both weights, for queries and for keys; angles reduced in fp64,
+// as rope_kernel) into shared memory, and a row then costs one scaling and four packed FMAs a
+// pair.  (Weights in registers and cos / sin alone in the table took 23 instructions an element,
+// 46.5 us for 8192 tokens of 40 heads of 128, against 25.6 us for the bytes.)  A row belongs to
+// GS = 2^k >= D / 16 threads with two 8-element vectors each, paired so that both halves of a NeoX
+// rotation are in one thread: vectors (u, u + rot_dim / 16) rotate, the rest pass through as
+// pairs with cos = 1; the sum of squares is reduced by shuffles.
 struct QkNormRopeParams {
     const uint4* q;
     const uint4* k;
@@ -312,12 +317,15 @@ struct QkNormRopeParams {
 };
 
 constexpr int kQkNormRopeTokens = 8;                       // the largest TPB
+constexpr int kQkNormRopePairs = 1024;                     // TPB * D / 2 at most
 
 template <bool BF16, bool NEOX>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormRopeParams p) {
+__global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(const QkNormRopeParams p) {
     constexpr int UNR = 4;                                 // rows a thread has in flight
+    // Pairs 2e, 2e + 1 of thread u, token t, queries (0) or keys (1): (A, A', B, B') and (C, C', S, S')
+    // at [kind][t][2e, 2e + 1][u]:  y0 = x0 A + x1 B,  y1 = x1 C + x0 S.
+    __shared__ float4 s_c[2 * kQkNormRopePairs];
     __shared__ double s_f[256];
-    __shared__ __align__(16) float s_cos[kQkNormRopeTokens * 256], s_sin[kQkNormRopeTokens * 256];
     __shared__ long long s_off[4][kQkNormRopeTokens];      // q, k, q_out, k_out offsets of each token
     __shared__ int s_pos[kQkNormRopeTokens];
     const int tid = threadIdx.x, half = p.rot_dim >> 1, H = p.H_q + p.H_kv;
@@ -341,109 +349,90 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormRopeParam
     const int end = min((split + 1) * p.rows_per_split, n_tok * H);
     int row = split * p.rows_per_split + rg;
     int tk = row / H, h = row - tk * H;
-    // The thread's two vectors, and the first pair index of their rotation (-1: they pass through).
-    int c0, c1, p0 = -1, p1 = -1;
-    if (NEOX) {
-        const int r = p.rot_dim >> 4;
-        c0 = u < r ? u : 2 * u;
-        c1 = u < r ? u + r : 2 * u + 1;
-        if (u < r) p0 = 8 * u;
-    } else {
-        c0 = u;
-        c1 = u + U;
-        if (8 * c0 < p.rot_dim) p0 = 4 * c0;
-        if (8 * c1 < p.rot_dim) p1 = 4 * c1;
-    }
+    const int r = p.rot_dim >> 4;
+    const int c0 = !NEOX || u < r ? u : 2 * u, c1 = !NEOX ? u + U : u < r ? u + r : 2 * u + 1;   // its vectors
     const bool on = u < U;
-    const uint4 one = pack8<BF16>({1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f});
-    uint4 w[2][2] = {{one, one}, {one, one}};
-    if (on && p.qw) { w[0][0] = __ldg(p.qw + c0); w[0][1] = __ldg(p.qw + c1); }
-    if (on && p.kw) { w[1][0] = __ldg(p.kw + c0); w[1][1] = __ldg(p.kw + c1); }
 
-    bool angles = false;
+    bool first = true;
     for (; row - rg < end; row += UNR * RG) {                            // (the same trips for the whole block)
         uint4 v[UNR][2];
         uint4* out[UNR];
-        int at[UNR];                                                     // token, or -1: no row
-        bool is_q[UNR];
+        int at[UNR];                                                     // the row's coefficients; -1: no row
 #pragma unroll
         for (int i = 0; i < UNR; ++i) {
             at[i] = -1;
             v[i][0] = v[i][1] = make_uint4(0u, 0u, 0u, 0u);
-            if (row + i * RG < end) {
-                at[i] = tk;
-                is_q[i] = h < p.H_q;
-                const uint4* src = is_q[i] ? p.q + s_off[0][tk] + h * p.q_sh : p.k + s_off[1][tk] + (h - p.H_q) * p.k_sh;
-                out[i] = is_q[i] ? p.qo + s_off[2][tk] + h * p.qo_sh : p.ko + s_off[3][tk] + (h - p.H_q) * p.ko_sh;
-                if (on) {
-                    v[i][0] = ld_stream(src + c0);
-                    v[i][1] = ld_stream(src + c1);
-                }
+            if (row + i * RG < end && on) {
+                const bool is_q = h < p.H_q;
+                const int hh = is_q ? h : h - p.H_q;
+                const uint4* src = (is_q ? p.q + s_off[0][tk] : p.k + s_off[1][tk]) + hh * (is_q ? p.q_sh : p.k_sh);
+                out[i] = (is_q ? p.qo + s_off[2][tk] : p.ko + s_off[3][tk]) + hh * (is_q ? p.qo_sh : p.ko_sh);
+                at[i] = ((is_q ? 0 : n_tok) + tk) * 8 * U + u;
+                v[i][0] = ld_stream(src + c0);
+                v[i][1] = ld_stream(src + c1);
             }
             for (h += RG; h >= H; h -= H) ++tk;
         }
-        if (!angles) {                                                   // while the first rows are on their way
-            for (int i = tid; i < n_tok * half; i += 256) {
-                const int t = i / half;
-                float sn, cs;
-                sincosf(reduce_2pi(s_pos[t] * s_f[i - t * half]), &sn, &cs);
-                s_cos[i] = cs * p.rot_scale;
-                s_sin[i] = sn * p.rot_scale;
+        if (first) {                                                     // while the first rows are on their way
+            first = false;
+            for (int i = tid; i < n_tok * 8 * U; i += 256) {
+                const int t = i / (8 * U), e = (i - t * 8 * U) / U, w = i - t * 8 * U - e * U;   // pair e of thread w
+                int i0, i1, pr;
+                if (NEOX) {
+                    i0 = w < r ? 8 * w + e : 16 * w + e;
+                    i1 = w < r ? i0 + half : i0 + 8;
+                    pr = w < r ? i0 : -1;
+                } else {
+                    i0 = 8 * (e < 4 ? w : w + U) + 2 * (e & 3);
+                    i1 = i0 + 1;
+                    pr = i0 < p.rot_dim ? i0 >> 1 : -1;
+                }
+                float sn = 0.f, cs = 1.f;
+                if (pr >= 0) {
+                    sincosf(reduce_2pi(s_pos[t] * s_f[pr]), &sn, &cs);
+                    sn *= p.rot_scale;
+                    cs *= p.rot_scale;
+                }
+#pragma unroll
+                for (int kind = 0; kind < 2; ++kind) {
+                    const uint16_t* wt = reinterpret_cast<const uint16_t*>(kind ? p.kw : p.qw);
+                    const float w0 = wt ? to_f32<BF16>(wt[i0]) : 1.f, w1 = wt ? to_f32<BF16>(wt[i1]) : 1.f;
+                    float* c = reinterpret_cast<float*>(s_c + ((kind * n_tok + t) * 8 + (e & ~1)) * U + w) + (e & 1);
+                    c[0] = w0 * cs;
+                    c[2] = -w1 * sn;
+                    c[4 * U] = w1 * cs;
+                    c[4 * U + 2] = w0 * sn;
+                }
             }
             __syncthreads();
-            angles = true;
         }
 #pragma unroll
         for (int i = 0; i < UNR; ++i) {
-            float x[2][8], ss = 0.f;
+            float x[2][8];
+            float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 unpack8<BF16>(v[i][c], x[c]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ss = fmaf(x[c][e], x[c][e], ss);
+                for (int e = 0; e < 8; e += 2) ss = ffma2(make_float2(x[c][e], x[c][e + 1]), make_float2(x[c][e], x[c][e + 1]), ss);
             }
-            for (int o = p.GS >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (at[i] < 0 || !on) continue;
-            const float r = rsqrtf(fmaf(ss, p.inv_D, p.eps));
+            float sum = ss.x + ss.y;
+            for (int o = p.GS >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (at[i] < 0) continue;
+            const float rinv = rsqrtf(fmaf(sum, p.inv_D, p.eps));
+            const float2 rr = make_float2(rinv, rinv);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float wt[8];
-                unpack8<BF16>(is_q[i] ? w[0][c] : w[1][c], wt);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[c][e] *= r * wt[e];
-            }
-            const float* cs = s_cos + at[i] * half;
-            const float* sn = s_sin + at[i] * half;
-            if (NEOX) {
-                if (p0 >= 0) {
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float4 c4 = *reinterpret_cast<const float4*>(cs + p0 + 4 * g);
-                        const float4 s4 = *reinterpret_cast<const float4*>(sn + p0 + 4 * g);
-                        const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, sc[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float a = x[0][4 * g + e], b = x[1][4 * g + e];
-                            x[0][4 * g + e] = fmaf(a, cc[e], -b * sc[e]);
-                            x[1][4 * g + e] = fmaf(b, cc[e], a * sc[e]);
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int pr = c ? p1 : p0;
-                    if (pr < 0) continue;
-                    const float4 c4 = *reinterpret_cast<const float4*>(cs + pr);
-                    const float4 s4 = *reinterpret_cast<const float4*>(sn + pr);
-                    const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, sc[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float a = x[c][2 * e], b = x[c][2 * e + 1];
-                        x[c][2 * e] = fmaf(a, cc[e], -b * sc[e]);
-                        x[c][2 * e + 1] = fmaf(b, cc[e], a * sc[e]);
-                    }
-                }
+            for (int e = 0; e < 8; e += 2) {
+                const float4 ab = s_c[at[i] + e * U], cd = s_c[at[i] + (e + 1) * U];
+                float* y[4];                                             // x0, x0', x1, x1' of the two pairs
+                y[0] = NEOX ? &x[0][e] : &x[e >> 2][2 * (e & 3)];
+                y[1] = NEOX ? &x[0][e + 1] : y[0] + 2;
+                y[2] = NEOX ? &x[1][e] : y[0] + 1;
+                y[3] = NEOX ? &x[1][e + 1] : y[0] + 3;
+                const float2 a = fmul2(make_float2(*y[0], *y[1]), rr), b = fmul2(make_float2(*y[2], *y[3]), rr);
+                const float2 o0 = ffma2(a, make_float2(ab.x, ab.y), fmul2(b, make_float2(ab.z, ab.w)));
+                const float2 o1 = ffma2(b, make_float2(cd.x, cd.y), fmul2(a, make_float2(cd.z, cd.w)));
+                *y[0] = o0.x; *y[1] = o0.y; *y[2] = o1.x; *y[3] = o1.y;
             }
             st_stream(out[i] + c0, pack8<BF16>(x[0]));
             st_stream(out[i] + c1, pack8<BF16>(x[1]));
