@@ -68,49 +68,57 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {
     return d;
 }
 
+// n / d for n < 2^31 by a multiplication: d <= 2^shift, mul = floor(2^32 (2^shift - d) / d) + 1.
+struct FastDiv {
+    unsigned mul, shift;
+    __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 struct Q4IoParams {
     uint8_t* cache;
     const int* slots;             // [B, S]
     uint4* k;
     uint4* v;
-    long long k_sb, k_sh, k_ss;   // strides in 16-byte vectors
-    long long v_sb, v_sh, v_ss;
-    long long n_tokens;           // B * S
+    unsigned k_sb, k_sh, k_ss;    // strides in 16-byte vectors
+    unsigned v_sb, v_sh, v_ss;
     int S, H;
+    unsigned rows;                // B * S * 2 H < 2^31
+    int head_major;               // order of a sequence's rows: head by head (K, then V), or token by token
+    int n_in, n_out;              // S and 2 H, or 2 H and S
+    FastDiv by_in, by_out;
+    int passes;                   // rows a thread takes, at most UNR
     int bs_log2;                  // log2(block_size)
-    int TPB;                      // tokens per block
-    int splits, rows_per_split;   // blocks per token group, and their rows (K and V of each head) of it
     long long n_slots;            // n_blocks * block_size
 };
 
-constexpr int kQ4IoTokens = 16;                            // the largest TPB
-
-// Both kernels below are bound by HBM.  A block takes a few tokens (their slots and offsets are
-// looked up once, in shared memory) and all their rows, K and V of each head; a thread has UNR
-// rows in flight.  Rows of one token are neighbours in the 16-bit tensors ([B, S, H, D]) or
-// (token by token) in their head ([B, H, S, D]): either way every access is whole sectors.
-struct Q4Tokens {
-    long long k[kQ4IoTokens], v[kQ4IoTokens];              // offsets in the 16-bit tensors, vectors
-    long long group[kQ4IoTokens];                          // byte offset of head 0's group; -1: no such slot
-    int row[kQ4IoTokens];                                  // row in it
+// Both kernels below are bound by HBM.  Rows are numbered as they lie in the 16-bit tensors: token
+// by token ([B, S, H, D]) or head by head ([B, H, S, D], where neighbours also share the cache's
+// groups).  A block takes up to four passes of neighbouring rows, all in flight; one pass where
+// that still leaves SMs idle.
+struct Q4Row {
+    bool is_v;
+    int h;
+    unsigned tok;
+    unsigned long long at;         // offset in the 16-bit tensor, vectors
 };
-
+__device__ __forceinline__ Q4Row q4_row(const Q4IoParams& p, unsigned row) {
+    Q4Row r;
+    const unsigned q = p.by_in.div(row), in = row - q * p.n_in, b = p.by_out.div(q), out = q - b * p.n_out;
+    const int hh = p.head_major ? out : in, s = p.head_major ? in : out;
+    r.tok = b * p.S + s;
+    r.is_v = hh >= p.H;
+    r.h = r.is_v ? hh - p.H : hh;
+    const unsigned sb = r.is_v ? p.v_sb : p.k_sb, sh = r.is_v ? p.v_sh : p.k_sh, ss = r.is_v ? p.v_ss : p.k_ss;
+    r.at = static_cast<unsigned long long>(b) * sb + static_cast<unsigned long long>(r.h) * sh +
+           static_cast<unsigned long long>(s) * ss;
+    return r;
+}
+// The group that holds `slot` of a head; nullptr outside the cache.
 template <int D>
-__device__ __forceinline__ int q4_tokens(const Q4IoParams& p, Q4Tokens& tok, long long tok0) {
-    const int n = p.n_tokens - tok0 < p.TPB ? static_cast<int>(p.n_tokens - tok0) : p.TPB;
-    const int tid = threadIdx.x;
-    if (tid < n) {
-        const long long t = tok0 + tid, b = t / p.S, s = t - b * p.S;
-        const long long slot = p.slots[t];
-        const long long groups = 1ll << (p.bs_log2 - 4);
-        tok.k[tid] = b * p.k_sb + s * p.k_ss;
-        tok.v[tid] = b * p.v_sb + s * p.v_ss;
-        tok.group[tid] = slot < 0 || slot >= p.n_slots
-                             ? -1 : ((slot >> p.bs_log2) * p.H * groups + ((slot >> 4) & (groups - 1))) * Q4<D>::GROUP;
-        tok.row[tid] = slot & 15;
-    }
-    __syncthreads();
-    return n;
+__device__ __forceinline__ uint8_t* q4_group(const Q4IoParams& p, int slot, int h) {
+    if (slot < 0 || slot >= p.n_slots) return nullptr;
+    const unsigned gs = p.bs_log2 - 4, block = static_cast<unsigned>(slot) >> p.bs_log2;   // (fewer than 2^32 groups)
+    return p.cache + static_cast<unsigned long long>(((block * p.H + h) << gs) + ((slot >> 4) & ((1u << gs) - 1))) * Q4<D>::GROUP;
 }
 
 // A row belongs to D / 16 threads with the vectors u and u + D / 16: a store of their words is a
@@ -118,64 +126,57 @@ __device__ __forceinline__ int q4_tokens(const Q4IoParams& p, Q4Tokens& tok, lon
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256, 3) q4_write_kernel(const Q4IoParams p) {
     constexpr int GS = D / 16, RG = 256 / GS, UNR = 4;
-    __shared__ Q4Tokens tok;
-    const int tid = threadIdx.x, u = tid % GS, H2 = 2 * p.H, split = blockIdx.x % p.splits;
-    const int n = q4_tokens<D>(p, tok, static_cast<long long>(blockIdx.x / p.splits) * p.TPB);
-    const int end = min((split + 1) * p.rows_per_split, n * H2);
-    const size_t head = static_cast<size_t>(Q4<D>::GROUP) << (p.bs_log2 - 4);   // bytes from a head to the next
-    int row = split * p.rows_per_split + tid / GS;
-    int t = row / H2, r = row - t * H2;                                  // token, row of it: K of each head, then V
-    for (; row - tid / GS < end; row += UNR * RG) {
-        uint4 x4[UNR][2];
-        uint8_t* dst[UNR];
-        int at[UNR];
+    const int u = threadIdx.x % GS;
+    const unsigned row0 = blockIdx.x * (p.passes * RG) + threadIdx.x / GS;
+    uint4 x4[UNR][2];
+    int slot[UNR], h[UNR];                                           // head; V's have bit 30 set
 #pragma unroll
-        for (int i = 0; i < UNR; ++i) {
-            dst[i] = nullptr;
-            x4[i][0] = x4[i][1] = make_uint4(0u, 0u, 0u, 0u);
-            if (row + i * RG < end && tok.group[t] >= 0) {
-                const bool is_v = r >= p.H;
-                const int h = is_v ? r - p.H : r;
-                const uint4* src = is_v ? p.v + tok.v[t] + h * p.v_sh : p.k + tok.k[t] + h * p.k_sh;
-                x4[i][0] = ld_stream(src + u);
-                x4[i][1] = ld_stream(src + u + GS);
-                dst[i] = p.cache + tok.group[t] + h * head + (is_v ? Q4<D>::V_CODES : 0);
-                at[i] = tok.row[t];
-                if (is_v) at[i] |= 16;
+    for (int i = 0; i < UNR; ++i) {
+        const unsigned row = row0 + i * RG;
+        slot[i] = -1;
+        h[i] = 0;
+        x4[i][0] = x4[i][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (i < p.passes && row < p.rows) {
+            const Q4Row r = q4_row(p, row);
+            const uint4* src = (r.is_v ? p.v : p.k) + r.at;
+            x4[i][0] = ld_stream(src + u);
+            x4[i][1] = ld_stream(src + u + GS);
+            slot[i] = p.slots[r.tok];
+            h[i] = r.is_v ? r.h | 1 << 30 : r.h;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < UNR; ++i) {
+        if (i >= p.passes) break;
+        float x[2][8], lo = 0.f, hi = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            unpack8<BF16>(x4[i][c], x[c]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                lo = fminf(lo, x[c][e]);
+                hi = fmax_nan(hi, x[c][e]);
             }
-            for (r += RG; r >= H2; r -= H2) ++t;
         }
 #pragma unroll
-        for (int i = 0; i < UNR; ++i) {
-            float x[2][8], lo = 0.f, hi = 0.f;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                unpack8<BF16>(x4[i][c], x[c]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    lo = fminf(lo, x[c][e]);
-                    hi = fmax_nan(hi, x[c][e]);
-                }
-            }
-#pragma unroll
-            for (int o = GS / 2; o > 0; o >>= 1) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            }
-            if (!dst[i]) continue;
-            float inv, zp;
-            const uint32_t word = q4_params(lo, hi, &inv, &zp);
-            const int rr = at[i] & 15;
-            uint32_t* w = reinterpret_cast<uint32_t*>(dst[i] + rr * Q4<D>::ROW);
-            if (word == kQ4BadRow) {
-                w[u] = w[u + GS] = 0u;
-            } else {
-                w[u] = q4_codes8(x[0], inv, zp);
-                w[u + GS] = q4_codes8(x[1], inv, zp);
-            }
-            if (u == 0)
-                reinterpret_cast<uint32_t*>(dst[i] + (at[i] & 16 ? Q4<D>::V_WORDS - Q4<D>::V_CODES : Q4<D>::K_WORDS))[rr] = word;
+        for (int o = GS / 2; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
+        const bool is_v = h[i] >> 30;
+        uint8_t* g = q4_group<D>(p, slot[i], h[i] & 0xFFFF);
+        if (!g) continue;
+        float inv, zp;
+        const uint32_t word = q4_params(lo, hi, &inv, &zp);
+        const int rr = slot[i] & 15;
+        uint32_t* w = reinterpret_cast<uint32_t*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW);
+        if (word == kQ4BadRow) {
+            w[u] = w[u + GS] = 0u;
+        } else {
+            w[u] = q4_codes8(x[0], inv, zp);
+            w[u + GS] = q4_codes8(x[1], inv, zp);
+        }
+        if (u == 0) reinterpret_cast<uint32_t*>(g + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS))[rr] = word;
     }
 }
 
@@ -204,51 +205,51 @@ __device__ __forceinline__ void q4_values8(uint32_t w, const float (&zc)[5], con
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256, 4) q4_read_kernel(const Q4IoParams p) {
     constexpr int GS = D / 16, RG = 256 / GS, UNR = 4;
-    __shared__ Q4Tokens tok;
-    const int tid = threadIdx.x, u = tid % GS, H2 = 2 * p.H, split = blockIdx.x % p.splits;
-    const int n = q4_tokens<D>(p, tok, static_cast<long long>(blockIdx.x / p.splits) * p.TPB);
-    const int end = min((split + 1) * p.rows_per_split, n * H2);
-    const size_t head = static_cast<size_t>(Q4<D>::GROUP) << (p.bs_log2 - 4);
-    int row = split * p.rows_per_split + tid / GS;
-    int t = row / H2, r = row - t * H2;
-    for (; row < end; row += UNR * RG) {
-        uint32_t w[UNR][2], word[UNR];
-        uint4* dst[UNR];
+    const int u = threadIdx.x % GS;
+    const unsigned row0 = blockIdx.x * (p.passes * RG) + threadIdx.x / GS;
+    uint32_t w[UNR][2], word[UNR];
+    uint4* dst[UNR];
+    int slot[UNR], h[UNR];                                           // head; V's have bit 30 set
 #pragma unroll
-        for (int i = 0; i < UNR; ++i) {
-            dst[i] = nullptr;
-            w[i][0] = w[i][1] = word[i] = 0u;
-            if (row + i * RG < end) {
-                const bool is_v = r >= p.H;
-                const int h = is_v ? r - p.H : r;
-                dst[i] = (is_v ? p.v + tok.v[t] + h * p.v_sh : p.k + tok.k[t] + h * p.k_sh) + u;
-                if (tok.group[t] >= 0) {
-                    const uint8_t* g = p.cache + tok.group[t] + h * head;
-                    const int rr = tok.row[t];
-                    const uint32_t* c = reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW) + u;
-                    w[i][0] = __ldg(c);
-                    w[i][1] = __ldg(c + GS);
-                    word[i] = __ldg(reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS)) + rr);
-                }
-            }
-            for (r += RG; r >= H2; r -= H2) ++t;
+    for (int i = 0; i < UNR; ++i) {
+        const unsigned row = row0 + i * RG;
+        dst[i] = nullptr;
+        slot[i] = -1;
+        h[i] = 0;
+        if (i < p.passes && row < p.rows) {
+            const Q4Row r = q4_row(p, row);
+            dst[i] = (r.is_v ? p.v : p.k) + r.at + u;
+            slot[i] = p.slots[r.tok];
+            h[i] = r.is_v ? r.h | 1 << 30 : r.h;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < UNR; ++i) {
+        w[i][0] = w[i][1] = word[i] = 0u;
+        if (const uint8_t* g = q4_group<D>(p, slot[i], h[i] & 0xFFFF)) {
+            const bool is_v = h[i] >> 30;
+            const int rr = slot[i] & 15;
+            const uint32_t* c = reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW) + u;
+            w[i][0] = __ldg(c);
+            w[i][1] = __ldg(c + GS);
+            word[i] = __ldg(reinterpret_cast<const uint32_t*>(g + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS)) + rr);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < UNR; ++i) {
+        if (!dst[i]) continue;
+        const float s = q4_scale(word[i]), z = __uint_as_float(0x4B000000u | (word[i] & 15u)) - 8388608.0f;
+        float zc[5], sc[5];
+#pragma unroll
+        for (int e = 0; e < 5; ++e) {
+            zc[e] = fmaf(z, static_cast<float>(1 << (4 * e)), 8388608.0f);
+            sc[e] = s * (1.0f / static_cast<float>(1 << (4 * e)));
         }
 #pragma unroll
-        for (int i = 0; i < UNR; ++i) {
-            if (!dst[i]) continue;
-            const float s = q4_scale(word[i]), z = __uint_as_float(0x4B000000u | (word[i] & 15u)) - 8388608.0f;
-            float zc[5], sc[5];
-#pragma unroll
-            for (int e = 0; e < 5; ++e) {
-                zc[e] = fmaf(z, static_cast<float>(1 << (4 * e)), 8388608.0f);
-                sc[e] = s * (1.0f / static_cast<float>(1 << (4 * e)));
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float x[8];
-                q4_values8(w[i][c], zc, sc, x);
-                st_stream(dst[i] + c * GS, pack8<BF16>(x));
-            }
+        for (int c = 0; c < 2; ++c) {
+            float x[8];
+            q4_values8(w[i][c], zc, sc, x);
+            st_stream(dst[i] + c * GS, pack8<BF16>(x));
         }
     }
 }

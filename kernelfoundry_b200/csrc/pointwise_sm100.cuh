@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 // ---- Query/key norm with RoPE ---------------------------------------------------
 // y = rnd(rot(x * rsqrt(mean(x^2) + eps) * w)) on every head row of Q and K.  Bound by HBM (each
 // element read once, written once); the rotation's angles are the same for all heads, so a block
-// takes whole tokens: while its first rows are on their way it computes each pair's four
+// takes groups of whole tokens: while a group's first rows are on their way it computes each pair's four
 // coefficients (cos and sin times both weights, for queries and for keys; angles reduced in fp64,
 // as rope_kernel) into shared memory, and a row then costs one scaling and four packed FMAs a
 // pair.  (Weights in registers and cos / sin alone in the table took 23 instructions an element,
@@ -305,13 +305,14 @@ struct QkNormRopeParams {
     const uint4* kw;
     const int* pos;               // [B, S] positions, nullptr: position = s
     const float* inv_freq;        // [rot_dim / 2], nullptr: theta^(-2i/rot_dim)
-    long long q_sb, q_sh, q_ss, k_sb, k_sh, k_ss;        // strides in 16-byte vectors
-    long long qo_sb, qo_sh, qo_ss, ko_sb, ko_sh, ko_ss;
+    unsigned q_sb, q_sh, q_ss, k_sb, k_sh, k_ss;         // strides in 16-byte vectors
+    unsigned qo_sb, qo_sh, qo_ss, ko_sb, ko_sh, ko_ss;
     long long n_tokens;           // B * S
     int S, H_q, H_kv, D, rot_dim;
     int GS;                       // threads per row, a power of two
-    int TPB;                      // tokens per block
-    int splits, rows_per_split;   // blocks per token group and their rows (a multiple of 256 / GS)
+    int TPB;                      // tokens per group
+    int splits, rows_per_split;   // parts of a group's rows, and their rows (a multiple of 256 / GS)
+    int items;                    // groups * splits, strided over by the blocks
     float eps, rot_scale, inv_D;
     double log2_theta;
 };
@@ -326,117 +327,128 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(const QkNormRopePa
     // at [kind][t][2e, 2e + 1][u]:  y0 = x0 A + x1 B,  y1 = x1 C + x0 S.
     __shared__ float4 s_c[2 * kQkNormRopePairs];
     __shared__ double s_f[256];
-    __shared__ long long s_off[4][kQkNormRopeTokens];      // q, k, q_out, k_out offsets of each token
-    __shared__ int s_pos[kQkNormRopeTokens];
+    // q, k, q_out, k_out offsets and position of each token, of this group and of the next
+    __shared__ unsigned long long s_off[2][4][kQkNormRopeTokens];
+    __shared__ int s_pos[2][kQkNormRopeTokens];
     const int tid = threadIdx.x, half = p.rot_dim >> 1, H = p.H_q + p.H_kv;
-    const int split = blockIdx.x % p.splits;
-    const long long tok0 = static_cast<long long>(blockIdx.x / p.splits) * p.TPB;
-    const int n_tok = p.n_tokens - tok0 < p.TPB ? static_cast<int>(p.n_tokens - tok0) : p.TPB;
-    if (tid < n_tok) {
-        const long long t = tok0 + tid, b = t / p.S, s = t - b * p.S;
-        s_off[0][tid] = b * p.q_sb + s * p.q_ss;
-        s_off[1][tid] = b * p.k_sb + s * p.k_ss;
-        s_off[2][tid] = b * p.qo_sb + s * p.qo_ss;
-        s_off[3][tid] = b * p.ko_sb + s * p.ko_ss;
-        s_pos[tid] = p.pos ? p.pos[t] : static_cast<int>(s);
-    }
+    auto tokens = [&](int item, int buf) {
+        const unsigned t = (item / p.splits) * p.TPB + tid;
+        if (tid >= p.TPB || t >= p.n_tokens) return;
+        const unsigned b = t / p.S, s = t - b * p.S;
+        auto at = [&](unsigned sb, unsigned ss) { return static_cast<unsigned long long>(b) * sb + static_cast<unsigned long long>(s) * ss; };
+        s_off[buf][0][tid] = at(p.q_sb, p.q_ss);
+        s_off[buf][1][tid] = at(p.k_sb, p.k_ss);
+        s_off[buf][2][tid] = at(p.qo_sb, p.qo_ss);
+        s_off[buf][3][tid] = at(p.ko_sb, p.ko_ss);
+        s_pos[buf][tid] = p.pos ? p.pos[t] : static_cast<int>(s);
+    };
+    tokens(blockIdx.x, 0);
     for (int i = tid; i < half; i += 256)
         s_f[i] = p.inv_freq ? static_cast<double>(p.inv_freq[i]) : exp2(-(2.0 * i / p.rot_dim) * p.log2_theta);
     __syncthreads();
 
     // row groups, this thread's, its place in the row, threads of a row that hold something
     const int RG = 256 / p.GS, rg = tid / p.GS, u = tid & (p.GS - 1), U = p.D >> 4;
-    const int end = min((split + 1) * p.rows_per_split, n_tok * H);
-    int row = split * p.rows_per_split + rg;
-    int tk = row / H, h = row - tk * H;
     const int r = p.rot_dim >> 4;
     const int c0 = !NEOX || u < r ? u : 2 * u, c1 = !NEOX ? u + U : u < r ? u + r : 2 * u + 1;   // its vectors
     const bool on = u < U;
 
-    bool first = true;
-    for (; row - rg < end; row += UNR * RG) {                            // (the same trips for the whole block)
-        uint4 v[UNR][2];
-        uint4* out[UNR];
-        int at[UNR];                                                     // the row's coefficients; -1: no row
+    int buf = 0;
+    for (int item = blockIdx.x; item < p.items; item += gridDim.x, buf ^= 1) {
+        const int group = item / p.splits, split = item - group * p.splits;
+        const int left = static_cast<int>(p.n_tokens) - group * p.TPB, n_tok = left < p.TPB ? left : p.TPB;
+        const int end = min((split + 1) * p.rows_per_split, n_tok * H);
+        int row = split * p.rows_per_split + rg;
+        int tk = row / H, h = row - tk * H;
+        bool first = true;
+        for (; row - rg < end; row += UNR * RG) {                            // (the same trips for the whole block)
+            uint4 v[UNR][2];
+            uint4* out[UNR];
+            int at[UNR];                                                     // the row's coefficients; -1: no row
 #pragma unroll
-        for (int i = 0; i < UNR; ++i) {
-            at[i] = -1;
-            v[i][0] = v[i][1] = make_uint4(0u, 0u, 0u, 0u);
-            if (row + i * RG < end && on) {
-                const bool is_q = h < p.H_q;
-                const int hh = is_q ? h : h - p.H_q;
-                const uint4* src = (is_q ? p.q + s_off[0][tk] : p.k + s_off[1][tk]) + hh * (is_q ? p.q_sh : p.k_sh);
-                out[i] = (is_q ? p.qo + s_off[2][tk] : p.ko + s_off[3][tk]) + hh * (is_q ? p.qo_sh : p.ko_sh);
-                at[i] = ((is_q ? 0 : n_tok) + tk) * 8 * U + u;
-                v[i][0] = ld_stream(src + c0);
-                v[i][1] = ld_stream(src + c1);
-            }
-            for (h += RG; h >= H; h -= H) ++tk;
-        }
-        if (first) {                                                     // while the first rows are on their way
-            first = false;
-            for (int i = tid; i < n_tok * 8 * U; i += 256) {
-                const int t = i / (8 * U), e = (i - t * 8 * U) / U, w = i - t * 8 * U - e * U;   // pair e of thread w
-                int i0, i1, pr;
-                if (NEOX) {
-                    i0 = w < r ? 8 * w + e : 16 * w + e;
-                    i1 = w < r ? i0 + half : i0 + 8;
-                    pr = w < r ? i0 : -1;
-                } else {
-                    i0 = 8 * (e < 4 ? w : w + U) + 2 * (e & 3);
-                    i1 = i0 + 1;
-                    pr = i0 < p.rot_dim ? i0 >> 1 : -1;
+            for (int i = 0; i < UNR; ++i) {
+                at[i] = -1;
+                v[i][0] = v[i][1] = make_uint4(0u, 0u, 0u, 0u);
+                if (row + i * RG < end && on) {
+                    const bool is_q = h < p.H_q;
+                    const unsigned hh = is_q ? h : h - p.H_q;
+                    const uint4* src = (is_q ? p.q : p.k) + s_off[buf][is_q ? 0 : 1][tk] +
+                                       static_cast<unsigned long long>(hh) * (is_q ? p.q_sh : p.k_sh);
+                    out[i] = (is_q ? p.qo : p.ko) + s_off[buf][is_q ? 2 : 3][tk] +
+                             static_cast<unsigned long long>(hh) * (is_q ? p.qo_sh : p.ko_sh);
+                    at[i] = ((is_q ? 0 : n_tok) + tk) * 8 * U + u;
+                    v[i][0] = ld_stream(src + c0);
+                    v[i][1] = ld_stream(src + c1);
                 }
-                float sn = 0.f, cs = 1.f;
-                if (pr >= 0) {
-                    sincosf(reduce_2pi(s_pos[t] * s_f[pr]), &sn, &cs);
-                    sn *= p.rot_scale;
-                    cs *= p.rot_scale;
+                for (h += RG; h >= H; h -= H) ++tk;
+            }
+            if (first) {                                                     // while the first rows are on their way
+                first = false;
+                for (int i = tid; i < n_tok * 8 * U; i += 256) {
+                    const int t = i / (8 * U), e = (i - t * 8 * U) / U, w = i - t * 8 * U - e * U;   // pair e of thread w
+                    int i0, i1, pr;
+                    if (NEOX) {
+                        i0 = w < r ? 8 * w + e : 16 * w + e;
+                        i1 = w < r ? i0 + half : i0 + 8;
+                        pr = w < r ? i0 : -1;
+                    } else {
+                        i0 = 8 * (e < 4 ? w : w + U) + 2 * (e & 3);
+                        i1 = i0 + 1;
+                        pr = i0 < p.rot_dim ? i0 >> 1 : -1;
+                    }
+                    float sn = 0.f, cs = 1.f;
+                    if (pr >= 0) {
+                        sincosf(reduce_2pi(s_pos[buf][t] * s_f[pr]), &sn, &cs);
+                        sn *= p.rot_scale;
+                        cs *= p.rot_scale;
+                    }
+#pragma unroll
+                    for (int kind = 0; kind < 2; ++kind) {
+                        const uint16_t* wt = reinterpret_cast<const uint16_t*>(kind ? p.kw : p.qw);
+                        const float w0 = wt ? to_f32<BF16>(wt[i0]) : 1.f, w1 = wt ? to_f32<BF16>(wt[i1]) : 1.f;
+                        float* c = reinterpret_cast<float*>(s_c + ((kind * n_tok + t) * 8 + (e & ~1)) * U + w) + (e & 1);
+                        c[0] = w0 * cs;
+                        c[2] = -w1 * sn;
+                        c[4 * U] = w1 * cs;
+                        c[4 * U + 2] = w0 * sn;
+                    }
                 }
+                if (item + static_cast<int>(gridDim.x) < p.items) tokens(item + gridDim.x, buf ^ 1);
+                __syncthreads();
+            }
 #pragma unroll
-                for (int kind = 0; kind < 2; ++kind) {
-                    const uint16_t* wt = reinterpret_cast<const uint16_t*>(kind ? p.kw : p.qw);
-                    const float w0 = wt ? to_f32<BF16>(wt[i0]) : 1.f, w1 = wt ? to_f32<BF16>(wt[i1]) : 1.f;
-                    float* c = reinterpret_cast<float*>(s_c + ((kind * n_tok + t) * 8 + (e & ~1)) * U + w) + (e & 1);
-                    c[0] = w0 * cs;
-                    c[2] = -w1 * sn;
-                    c[4 * U] = w1 * cs;
-                    c[4 * U + 2] = w0 * sn;
+            for (int i = 0; i < UNR; ++i) {
+                float x[2][8];
+                float2 ss = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    unpack8<BF16>(v[i][c], x[c]);
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) ss = ffma2(make_float2(x[c][e], x[c][e + 1]), make_float2(x[c][e], x[c][e + 1]), ss);
                 }
+                float sum = ss.x + ss.y;
+                for (int o = p.GS >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (at[i] < 0) continue;
+                const float rinv = rsqrtf(fmaf(sum, p.inv_D, p.eps));
+                const float2 rr = make_float2(rinv, rinv);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const float4 ab = s_c[at[i] + e * U], cd = s_c[at[i] + (e + 1) * U];
+                    float* y[4];                                             // x0, x0', x1, x1' of the two pairs
+                    y[0] = NEOX ? &x[0][e] : &x[e >> 2][2 * (e & 3)];
+                    y[1] = NEOX ? &x[0][e + 1] : y[0] + 2;
+                    y[2] = NEOX ? &x[1][e] : y[0] + 1;
+                    y[3] = NEOX ? &x[1][e + 1] : y[0] + 3;
+                    const float2 a = fmul2(make_float2(*y[0], *y[1]), rr), b = fmul2(make_float2(*y[2], *y[3]), rr);
+                    const float2 o0 = ffma2(a, make_float2(ab.x, ab.y), fmul2(b, make_float2(ab.z, ab.w)));
+                    const float2 o1 = ffma2(b, make_float2(cd.x, cd.y), fmul2(a, make_float2(cd.z, cd.w)));
+                    *y[0] = o0.x; *y[1] = o0.y; *y[2] = o1.x; *y[3] = o1.y;
+                }
+                st_stream(out[i] + c0, pack8<BF16>(x[0]));
+                st_stream(out[i] + c1, pack8<BF16>(x[1]));
             }
-            __syncthreads();
         }
-#pragma unroll
-        for (int i = 0; i < UNR; ++i) {
-            float x[2][8];
-            float2 ss = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                unpack8<BF16>(v[i][c], x[c]);
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) ss = ffma2(make_float2(x[c][e], x[c][e + 1]), make_float2(x[c][e], x[c][e + 1]), ss);
-            }
-            float sum = ss.x + ss.y;
-            for (int o = p.GS >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (at[i] < 0) continue;
-            const float rinv = rsqrtf(fmaf(sum, p.inv_D, p.eps));
-            const float2 rr = make_float2(rinv, rinv);
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float4 ab = s_c[at[i] + e * U], cd = s_c[at[i] + (e + 1) * U];
-                float* y[4];                                             // x0, x0', x1, x1' of the two pairs
-                y[0] = NEOX ? &x[0][e] : &x[e >> 2][2 * (e & 3)];
-                y[1] = NEOX ? &x[0][e + 1] : y[0] + 2;
-                y[2] = NEOX ? &x[1][e] : y[0] + 1;
-                y[3] = NEOX ? &x[1][e + 1] : y[0] + 3;
-                const float2 a = fmul2(make_float2(*y[0], *y[1]), rr), b = fmul2(make_float2(*y[2], *y[3]), rr);
-                const float2 o0 = ffma2(a, make_float2(ab.x, ab.y), fmul2(b, make_float2(ab.z, ab.w)));
-                const float2 o1 = ffma2(b, make_float2(cd.x, cd.y), fmul2(a, make_float2(cd.z, cd.w)));
-                *y[0] = o0.x; *y[1] = o0.y; *y[2] = o1.x; *y[3] = o1.y;
-            }
-            st_stream(out[i] + c0, pack8<BF16>(x[0]));
-            st_stream(out[i] + c1, pack8<BF16>(x[1]));
-        }
+        __syncthreads();                                                 // the coefficients are free
     }
 }
 
