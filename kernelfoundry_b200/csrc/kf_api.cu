@@ -1480,12 +1480,11 @@ int kf_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
     p.rot_dim = rot_dim;
     p.GS = 1;
     while (p.GS < D / 16) p.GS <<= 1;
-    // Groups of tokens: small ones spread evenly over the blocks (8192 tokens: 4 a group 36.1 us,
-    // 8 38.4), but where there are fewer tokens than blocks the rows of a token are split.
+    // Groups of tokens: as large as leave two an SM (2331 tokens of 15 heads of 256: 4 a group 11.0 us,
+    // 8 13.0, 1 24); where there are fewer tokens than that the rows of a token are split.
     const int H = H_q + H_kv, rows_at_once = 256 / p.GS, sms = di->sm_count;
     p.TPB = kf::kQkNormRopeTokens;
     while (p.TPB > 1 && (p.TPB * (D / 2) > kf::kQkNormRopePairs || n_tokens < 2ll * sms * p.TPB)) p.TPB >>= 1;
-    if (const char* e = std::getenv("KF_RTPB")) p.TPB = std::atoi(e);
     const int passes = (p.TPB * H + rows_at_once - 1) / rows_at_once;
     int splits = p.TPB > 1 || n_tokens >= 2 * sms ? 1 : static_cast<int>(2 * sms / n_tokens);
     if (splits > passes) splits = passes;

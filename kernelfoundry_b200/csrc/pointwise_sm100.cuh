@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 // y = rnd(rot(x * rsqrt(mean(x^2) + eps) * w)) on every head row of Q and K.  Bound by HBM (each
 // element read once, written once); the rotation's angles are the same for all heads, so a block
 // takes groups of whole tokens: while a group's first rows are on their way it computes each pair's four
-// coefficients (cos and sin times both weights, for queries and for keys; angles reduced in fp64,
-// as rope_kernel) into shared memory, and a row then costs one scaling and four packed FMAs a
+// coefficients (cos and sin times both weights, for queries and for keys; angles in half turns,
+// reduced in fp64) into shared memory, and a row then costs one scaling and four packed FMAs a
 // pair.  (Weights in registers and cos / sin alone in the table took 23 instructions an element,
 // 46.5 us for 8192 tokens of 40 heads of 128, against 25.6 us for the bytes.)  A row belongs to
 // GS = 2^k >= D / 16 threads with two 8-element vectors each, paired so that both halves of a NeoX
@@ -321,8 +321,8 @@ constexpr int kQkNormRopeTokens = 8;                       // the largest TPB
 constexpr int kQkNormRopePairs = 1024;                     // TPB * D / 2 at most
 
 template <bool BF16, bool NEOX>
-__global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(const QkNormRopeParams p) {
-    constexpr int UNR = 4;                                 // rows a thread has in flight
+__global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const QkNormRopeParams p) {
+    constexpr int UNR = 2;                                 // rows a thread has in flight (4: fewer warps fit, 40 us)
     // Pairs 2e, 2e + 1 of thread u, token t, queries (0) or keys (1): (A, A', B, B') and (C, C', S, S')
     // at [kind][t][2e, 2e + 1][u]:  y0 = x0 A + x1 B,  y1 = x1 C + x0 S.
     __shared__ float4 s_c[2 * kQkNormRopePairs];
@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(const QkNormRopePa
     };
     tokens(blockIdx.x, 0);
     for (int i = tid; i < half; i += 256)
-        s_f[i] = p.inv_freq ? static_cast<double>(p.inv_freq[i]) : exp2(-(2.0 * i / p.rot_dim) * p.log2_theta);
+        s_f[i] = 0.3183098861837907 *                      // half turns per position
+                 (p.inv_freq ? static_cast<double>(p.inv_freq[i]) : exp2(-(2.0 * i / p.rot_dim) * p.log2_theta));
     __syncthreads();
 
     // row groups, this thread's, its place in the row, threads of a row that hold something
@@ -398,7 +399,8 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(const QkNormRopePa
                     }
                     float sn = 0.f, cs = 1.f;
                     if (pr >= 0) {
-                        sincosf(reduce_2pi(s_pos[buf][t] * s_f[pr]), &sn, &cs);
+                        const double a = s_pos[buf][t] * s_f[pr];
+                        sincospif(static_cast<float>(a - 2.0 * rint(0.5 * a)), &sn, &cs);
                         sn *= p.rot_scale;
                         cs *= p.rot_scale;
                     }
