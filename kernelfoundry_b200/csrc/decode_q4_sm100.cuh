@@ -19,8 +19,9 @@
 // Queries are scaled by a power of two per row to a maximum in [2^13, 2^14), which holds fp16
 // rows exactly, and bf16 ones but for elements below 2^-28 of the row's largest.
 // p t enters the second product as fp16, scaled by a power of two such that the largest t seen
-// stays below 2^7 (t spans any range; small ones lose bits only against the largest).  This
-// rounding, 2^-11 relative per key, is the only one below fp32 in the sum.
+// stays below 2^7 (t spans any range; small ones lose bits only against the largest).  For a
+// bf16 output this rounding, 2^-11 relative per key, is the only one below fp32 in the sum; for
+// fp16 and fp32 outputs (SPLIT) what it leaves goes in as a second fp16 operand, which leaves 2^-22.
 // The running maximum is lazy: p = 2^(x - m) with an m that is raised only when a score passes
 // m + 8 (p <= 2^8 then, which fp16 and fp32 hold as well as p <= 1), so a tile needs one vote
 // instead of a maximum across the warp.  The true maximum is kept per thread and put in at the end.
@@ -116,14 +117,15 @@ struct Q4Cursor {
     int nt, len;                   // the sequence's tiles and keys
 };
 
+constexpr float kQ4NoMax = -1e30f;
+
 template <int D, int NT>
 struct Q4Warp {                    // a warp's running state of one unit; pairs: columns 2t, 2t + 1
     float o[NT][Q4AttnCfg<D, NT>::MT][4];
-    float2 m[NT], ms[NT], l[NT];   // reference of the exponent (ms: 0 while it is -inf), sum of p
+    float2 m[NT], l[NT];           // reference of the exponent (kQ4NoMax before the first key), sum of p
     float2 mt[NT];                 // this thread's largest score
     uint32_t q[NT][Q4AttnCfg<D, NT>::KW][4];
     float2 cq[NT];                 // a column's factor of the scores
-    int lim[NT][2];                // keys the column's query sees
     float tmx;                     // this thread's largest value scale
     float tlim, tnorm, tinv;       // value scales up to tlim times tnorm stay below 2^7; tinv = 1 / tnorm
 };
@@ -201,11 +203,9 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
         const float cq = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(ex - 13) << 23) * 0x1p9f;
         s.cq[n].x = __shfl_sync(0xffffffffu, cq, 8 * t);
         s.cq[n].y = __shfl_sync(0xffffffffu, cq, 8 * t + 4);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            s.lim[n][k] = c.len - (p.causal ? p.S_q - 1 - (c.rg * C::ROWS + 8 * n + 2 * t + k) % p.S_q : 0);
-        s.m[n] = s.mt[n] = make_float2(-INFINITY, -INFINITY);
-        s.ms[n] = s.l[n] = make_float2(0.f, 0.f);
+        s.m[n] = make_float2(kQ4NoMax, kQ4NoMax);
+        s.mt[n] = make_float2(-INFINITY, -INFINITY);
+        s.l[n] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < C::MT; ++i)
 #pragma unroll
@@ -215,10 +215,19 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
 
 // One tile of 32 keys from shared memory.  MASKED: some key is outside the sequence, hidden
 // from a row, or in a page outside the pool (valid: bit j set when group j was copied).
-template <int D, int NT, bool MASKED>
-__device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int key0, int len, uint32_t valid, int lane) {
+template <int D, int NT, bool SPLIT, bool MASKED>
+__device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s, const uint8_t* st, const Q4Cursor& c,
+                                        uint32_t valid, int lane) {
     using C = Q4AttnCfg<D, NT>;
-    const int g = lane >> 2, t = lane & 3;
+    const int g = lane >> 2, t = lane & 3, key0 = c.tile * 32, len = c.len;
+    int lim[NT][2];                // keys the column's query sees
+    if (MASKED) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                lim[n][k] = len - (p.causal ? p.S_q - 1 - (c.rg * C::ROWS + 8 * n + 2 * t + k) % p.S_q : 0);
+    }
     float2 x[2][NT][2];            // scores [group][query tile][row g or g + 8]
     float tv[2][2];                // value scales of the same rows
     // S^T = K Q^T, in two chains per 128 dims, added up in fp32
@@ -279,8 +288,8 @@ __device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int
                 float2 v = fmul2(x[j][n][h], fmul2(make_float2(sc, sc), s.cq[n]));
                 if (MASKED) {
                     if (!((valid >> j) & 1u)) v = make_float2(0.f, 0.f);     // a page outside the pool reads zeros
-                    if (key >= s.lim[n][0]) v.x = -INFINITY;
-                    if (key >= s.lim[n][1]) v.y = -INFINITY;
+                    if (key >= lim[n][0]) v.x = -INFINITY;
+                    if (key >= lim[n][1]) v.y = -INFINITY;
                 }
                 x[j][n][h] = v;
             }
@@ -310,17 +319,16 @@ __device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float v[2] = {s.mt[n].x, s.mt[n].y}, a[2];
-            float m[2] = {s.m[n].x, s.m[n].y}, ms[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
+                const float m = k ? s.m[n].y : s.m[n].x;
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 4));
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 8));
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 16));
-                ms[k] = v[k] == -INFINITY ? 0.f : v[k];
-                a[k] = ex2_approx(m[k] - ms[k]);
+                v[k] = fmaxf(v[k], m);                                       // (no key seen by this column yet: kQ4NoMax)
+                a[k] = ex2_approx(m - v[k]);
             }
             s.m[n] = make_float2(v[0], v[1]);
-            s.ms[n] = make_float2(ms[0], ms[1]);
             s.l[n] = make_float2(s.l[n].x * a[0], s.l[n].y * a[1]);
             a[0] *= r;
             a[1] *= r;
@@ -338,22 +346,28 @@ __device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int
     for (int j = 0; j < 2; ++j) {
         const uint8_t* gr = st + j * C::GROUP;
         const uint32_t* words = reinterpret_cast<const uint32_t*>(gr + Q4<D>::V_WORDS);
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][2], pl[NT][2];                                       // p t, and (SPLIT) what its rounding left
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const float tn = tv[j][h] * s.tnorm;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float2 d = fadd2(x[j][n][h], make_float2(-s.ms[n].x, -s.ms[n].y));
+                const float2 d = fadd2(x[j][n][h], make_float2(-s.m[n].x, -s.m[n].y));
                 const float2 pr = make_float2(ex2_approx(d.x), ex2_approx(d.y));
                 s.l[n] = fadd2(s.l[n], pr);
                 float2 pt = fmul2(pr, make_float2(tn, tn));
                 if (MASKED) {                                                // 0 * a spoiled row's NaN
                     const int key = key0 + 16 * j + 8 * h + g;
-                    if (key >= s.lim[n][0]) pt.x = 0.f;
-                    if (key >= s.lim[n][1]) pt.y = 0.f;
+                    if (key >= lim[n][0]) pt.x = 0.f;
+                    if (key >= lim[n][1]) pt.y = 0.f;
                 }
-                pb[n][h] = movmatrix_trans(pack_half2(pt.x, pt.y));
+                const uint32_t hi = pack_half2(pt.x, pt.y);
+                pb[n][h] = movmatrix_trans(hi);
+                if (SPLIT) {
+                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                    const float2 lo = fadd2(pt, make_float2(-back.x, -back.y));
+                    pl[n][h] = movmatrix_trans(pack_half2(lo.x, lo.y));
+                }
             }
         }
         const uint2 z01 = *reinterpret_cast<const uint2*>(words + 2 * t);
@@ -375,7 +389,10 @@ __device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_16816(s.o[n][i], a0[i], a1[i], a2[i], a3[i], pb[n][0], pb[n][1]);
+                for (int n = 0; n < NT; ++n) {
+                    mma_16816(s.o[n][i], a0[i], a1[i], a2[i], a3[i], pb[n][0], pb[n][1]);
+                    if (SPLIT) mma_16816(s.o[n][i], a0[i], a1[i], a2[i], a3[i], pl[n][0], pl[n][1]);
+                }
         } else {
 #pragma unroll
             for (int set = 0; set < C::SETS; ++set) {
@@ -395,8 +412,11 @@ __device__ __forceinline__ void q4_tile(Q4Warp<D, NT>& s, const uint8_t* st, int
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            mma_16816(s.o[n][set * 8 + q * 4 + i], a0[i], a1[i], a2[i], a3[i], pb[n][0], pb[n][1]);
+                        for (int n = 0; n < NT; ++n) {
+                            float(&o)[4] = s.o[n][set * 8 + q * 4 + i];
+                            mma_16816(o, a0[i], a1[i], a2[i], a3[i], pb[n][0], pb[n][1]);
+                            if (SPLIT) mma_16816(o, a0[i], a1[i], a2[i], a3[i], pl[n][0], pl[n][1]);
+                        }
                 }
             }
         }
@@ -562,7 +582,7 @@ __device__ __forceinline__ void q4_write(const Q4AttnParams& p, const Q4Merged<D
     if (r.stats && p.Li) p.Li[at] = r.L;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool SPLIT>
 __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(const __grid_constant__ Q4AttnParams p) {
     using C = Q4AttnCfg<D, NT>;
     constexpr int W = C::W, STAGES = C::STAGES;
@@ -660,11 +680,9 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         // every 32 tiles; the table entries of the next one are loaded when it does (a load waits
         // behind the copies in flight for microseconds).
         int issued = y0, win0 = y0;
-        const uint8_t* src0 = nullptr;
-        const uint8_t* src1 = nullptr;                                   // 16-token pages: the second group's
-        uint32_t bytes = 0, valid = 0;
+        unsigned f0 = 0, f1 = 0, f_at = 0, valid = 0;                    // the window's entries, and which are in the pool
         const bool paired = p.bs_log2 == 4;
-        unsigned e0 = 0, e1 = 0, e_at = 0;                               // entries to come, (head << 4 | group in the page), groups
+        unsigned e0 = 0, e1 = 0, e_at = 0;                               // the next one's; at: head << 4 | group in the page
         auto fetch = [&](int y) {                                        // for the window that begins at tile y
             e0 = e1 = 0xffffffffu;
             if (y + lane < y1) {
@@ -694,24 +712,27 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         };
         auto move_on = [&](int y) {
             win0 = y;
-            const bool v0 = e0 < static_cast<unsigned>(p.n_blocks), v1 = e1 < static_cast<unsigned>(p.n_blocks);
-            const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
-            src0 = p.cache + static_cast<uint64_t>(e0 * p.H_kv + (e_at >> 4)) * page_bytes + (e_at & 15u) * C::GROUP;
-            src1 = p.cache + static_cast<uint64_t>(e1 * p.H_kv + (e_at >> 4)) * page_bytes;
-            bytes = ((v0 ? 1u : 0u) + (v1 ? 1u : 0u)) * C::GROUP;
-            valid = (v0 ? 1u : 0u) | (v1 ? 2u : 0u);
+            f0 = e0;
+            f1 = e1;
+            f_at = e_at;
+            valid = (e0 < static_cast<unsigned>(p.n_blocks) ? 1u : 0u) | (e1 < static_cast<unsigned>(p.n_blocks) ? 2u : 0u);
             if (win0 + 32 < y1) fetch(win0 + 32);
         };
         auto issue = [&](int stage) {                                    // by the lane that holds the tile
             uint64_t* bar = &bars[warp][stage];
             uint8_t* dst = ring + stage * C::STAGE_BYTES;
+            const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
+            const uint32_t bytes = __popc(valid) * C::GROUP;
+            auto src = [&](unsigned e) {
+                return p.cache + static_cast<uint64_t>(e * p.H_kv + (f_at >> 4)) * page_bytes + (f_at & 15u) * C::GROUP;
+            };
             s_valid[warp][stage] = valid;
             mbar_arrive_expect_tx(bar, bytes);
             if (!paired) {
-                if (bytes) bulk_g2s(dst, src0, bytes, bar);              // both groups lie in one page
+                if (valid) bulk_g2s(dst, src(f0), bytes, bar);           // both groups lie in one page
             } else {
-                if (valid & 1u) bulk_g2s(dst, src0, C::GROUP, bar);
-                if (valid & 2u) bulk_g2s(dst + C::GROUP, src1, C::GROUP, bar);
+                if (valid & 1u) bulk_g2s(dst, src(f0), C::GROUP, bar);
+                if (valid & 2u) bulk_g2s(dst + C::GROUP, src(f1), C::GROUP, bar);
             }
         };
 
@@ -745,10 +766,9 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                     break;
                 }
                 const uint32_t got = s_valid[warp][stage];
-                const int key0 = cur.tile * 32;
                 const uint8_t* st = ring + stage * C::STAGE_BYTES;
-                if (got != 3u || key0 > plain_end) q4_tile<D, NT, true>(s, st, key0, cur.len, got, lane);
-                else q4_tile<D, NT, false>(s, st, key0, cur.len, got, lane);
+                if (got != 3u || cur.tile * 32 > plain_end) q4_tile<D, NT, SPLIT, true>(p, s, st, cur, got, lane);
+                else q4_tile<D, NT, SPLIT, false>(p, s, st, cur, got, lane);
                 ++cur.tile;
                 ++y_cur;
                 __syncwarp();

@@ -1557,11 +1557,14 @@ int q4_attn_launch(const kf::Q4AttnParams& p, long long max_tiles, int sm_count,
     using C = kf::Q4AttnCfg<D, NT>;
     static_assert(C::PART_FLOATS == 8 * NT * (D + 2), "part size");
     int bps = 0;
-    const int rc = kernel_setup<kf::q4_attn_kernel<D, NT>>(C::SMEM_BYTES, C::THREADS, &bps);
+    const bool split = p.out_type != kf::KF_OUT_BF16;
+    const int rc = split ? kernel_setup<kf::q4_attn_kernel<D, NT, true>>(C::SMEM_BYTES, C::THREADS, &bps)
+                         : kernel_setup<kf::q4_attn_kernel<D, NT, false>>(C::SMEM_BYTES, C::THREADS, &bps);
     if (rc != KF_OK) return rc;
     const long long want = (max_tiles + C::W - 1) / C::W;
     const unsigned grid = static_cast<unsigned>(want < sm_count ? want : sm_count);
-    const cudaError_t e = launch_pdl(kf::q4_attn_kernel<D, NT>, dim3(grid), C::THREADS, C::SMEM_BYTES, s, p);
+    const cudaError_t e = split ? launch_pdl(kf::q4_attn_kernel<D, NT, true>, dim3(grid), C::THREADS, C::SMEM_BYTES, s, p)
+                                : launch_pdl(kf::q4_attn_kernel<D, NT, false>, dim3(grid), C::THREADS, C::SMEM_BYTES, s, p);
     return e == cudaSuccess ? KF_OK : cuda_fail(e);
 }
 
