@@ -64,7 +64,7 @@ template <int D_, int NT_>
 struct Q4AttnCfg {
     static constexpr int D = D_, NT = NT_;
     static constexpr int W = D == 256 ? 8 : NT == 1 ? (D == 64 ? 16 : 12) : (D == 64 ? 12 : 8);   // warps
-    static constexpr int STAGES = D == 256 ? 2 : D == 64 ? 4 : NT == 1 ? 3 : 4;
+    static constexpr int STAGES = D == 256 ? 2 : D == 64 ? 4 : NT == 1 ? 2 : 4;
     static constexpr int THREADS = 32 * W;
     static constexpr int GROUP = Q4<D>::GROUP;
     static constexpr int STAGE_BYTES = 2 * GROUP;                // a tile: 32 keys
@@ -517,7 +517,7 @@ template <int D, int NT, bool GLOBAL>
 __device__ __forceinline__ Q4Merged<D, NT> q4_merge(int idx, int count, const float* first, const float* mid, size_t stride,
                                                     const float* last) {
     using C = Q4AttnCfg<D, NT>;
-    constexpr int U = GLOBAL ? 8 : 4;                                    // parts in flight
+    constexpr int U = GLOBAL ? (C::V4 == 1 ? 16 : 10) : 4;               // parts in flight
     const int ln = idx & 31, item = idx >> 5;
     const int e = item & 3, set = (item >> 2) % C::SETS, n = item / (4 * C::SETS);
     Q4Merged<D, NT> r;
@@ -803,7 +803,10 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     __syncthreads();
 
     // ---- merge the CTA's parts: runs of equal units in the entries' order
-    constexpr int items = NT * C::SETS * 4;
+    constexpr int items = NT * C::SETS * 4;                              // warps that merge a run
+    constexpr int teams = W / items > 0 ? W / items : 1;                 // runs merged side by side
+    const int team = warp / items, in_team = tid - team * items * 32;
+    int run_no = 0;
     const Q4Unit mine_u = lane < 2 * W ? s_ent[lane] : Q4Unit{-1, 0, 0};
     int cross_u[2] = {-1, -1}, cross_first[2] = {0, 0}, cross_n[2] = {0, 0};
     for (uint32_t todo = __ballot_sync(0xffffffffu, mine_u.u >= 0); todo;) {
@@ -822,8 +825,10 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         const bool inside = us >= x0 && us + unt <= x1;
         const int slot = us >= x0 ? 1 : 0;
         float* out = p.parts + (static_cast<size_t>(blockIdx.x) * 2 + slot) * C::PART_FLOATS;
+        const bool ours = teams == 1 || run_no % teams == team;
+        ++run_no;
 #pragma unroll 1
-        for (int idx = tid; idx < items * 32; idx += C::THREADS) {
+        for (int idx = teams == 1 ? tid : in_team; ours && idx < items * 32; idx += teams == 1 ? C::THREADS : items * 32) {
             const Q4Merged<D, NT> r = q4_merge<D, NT, false>(idx, count, entry(lead), entry(lead | 1),
                                                              STAGES * C::STAGE_BYTES / 4, entry(end));
             if (inside) {
@@ -857,26 +862,24 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
 
     // ---- units that cross CTAs: the last CTA to arrive merges the parts, in CTA order
     __syncthreads();
-    if (tid == 0) {                                                      // (its release covers what the barrier ordered before)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            s_last[k] = 0;
-            if (cross_u[k] >= 0 &&
-                atom_add_acq_rel_gpu(p.tickets + cross_first[k], 1u) == static_cast<unsigned>(cross_n[k] - 1)) {
-                p.tickets[cross_first[k]] = 0u;
-                s_last[k] = 1;
-            }
+    if (warp < 2 && lane == 0) {                                         // (its release covers what the barrier ordered before)
+        const int u = warp ? cross_u[1] : cross_u[0], first = warp ? cross_first[1] : cross_first[0];
+        const unsigned others = (warp ? cross_n[1] : cross_n[0]) - 1;
+        s_last[warp] = 0;
+        if (u >= 0 && atom_add_acq_rel_gpu(p.tickets + first, 1u) == others) {
+            p.tickets[first] = 0u;
+            s_last[warp] = 1;
         }
     }
     __syncthreads();
 #pragma unroll 1
     for (int k = 0; k < 2; ++k) {
-        if (!s_last[k]) continue;
+        if (!s_last[k] || (teams > 1 && team != k)) continue;
         const int cf = k ? cross_first[1] : cross_first[0], u = k ? cross_u[1] : cross_u[0];
         const int count = k ? cross_n[1] : cross_n[0];
         const float* mid = p.parts + static_cast<size_t>(cf) * 2 * C::PART_FLOATS;   // its first CTA's second slot, then first slots
 #pragma unroll 1
-        for (int idx = tid; idx < items * 32; idx += C::THREADS)
+        for (int idx = teams == 1 ? tid : in_team; idx < items * 32; idx += teams == 1 ? C::THREADS : items * 32)
             q4_write(p, q4_merge<D, NT, true>(idx, count, mid + C::PART_FLOATS, mid, 2 * C::PART_FLOATS,
                                               mid + (count - 1) * 2 * C::PART_FLOATS), u);
     }
