@@ -87,6 +87,14 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
+// mma_16816 with a zero C.
+__device__ __forceinline__ void mma_16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t hfma2_u(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -253,10 +261,6 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
             }
             float acc[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[0][n][e] = acc[1][n][e] = 0.f;
-#pragma unroll
             for (int i = 0; i < NW; ++i) {
                 const int w = hf * 4 + i;
                 const uint32_t ua = wa[i] >> 8, ub = wb[i] >> 8;
@@ -264,8 +268,13 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
                 const uint32_t c0 = q4_lo(ua, za), c1 = q4_lo(ub, zb), c2 = q4_hi(ua, za), c3 = q4_hi(ub, zb);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma_16816(acc[0][n], a0, a1, a2, a3, s.q[n][w][0], s.q[n][w][1]);
-                    mma_16816(acc[1][n], c0, c1, c2, c3, s.q[n][w][2], s.q[n][w][3]);
+                    if (i == 0) {
+                        mma_16816_first(acc[0][n], a0, a1, a2, a3, s.q[n][w][0], s.q[n][w][1]);
+                        mma_16816_first(acc[1][n], c0, c1, c2, c3, s.q[n][w][2], s.q[n][w][3]);
+                    } else {
+                        mma_16816(acc[0][n], a0, a1, a2, a3, s.q[n][w][0], s.q[n][w][1]);
+                        mma_16816(acc[1][n], c0, c1, c2, c3, s.q[n][w][2], s.q[n][w][3]);
+                    }
                 }
             }
 #pragma unroll
@@ -680,7 +689,9 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         // every 32 tiles; the table entries of the next one are loaded when it does (a load waits
         // behind the copies in flight for microseconds).
         int issued = y0, win0 = y0;
-        unsigned f0 = 0, f1 = 0, f_at = 0, valid = 0;                    // the window's entries, and which are in the pool
+        const uint8_t* src0 = nullptr;                                   // the window's groups, and which are in the pool
+        const uint8_t* src1 = nullptr;
+        uint32_t bytes = 0, valid = 0;
         const bool paired = p.bs_log2 == 4;
         unsigned e0 = 0, e1 = 0, e_at = 0;                               // the next one's; at: head << 4 | group in the page
         auto fetch = [&](int y) {                                        // for the window that begins at tile y
@@ -712,27 +723,23 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         };
         auto move_on = [&](int y) {
             win0 = y;
-            f0 = e0;
-            f1 = e1;
-            f_at = e_at;
+            const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
+            src0 = p.cache + static_cast<uint64_t>(e0 * p.H_kv + (e_at >> 4)) * page_bytes + (e_at & 15u) * C::GROUP;
+            src1 = p.cache + static_cast<uint64_t>(e1 * p.H_kv + (e_at >> 4)) * page_bytes;
             valid = (e0 < static_cast<unsigned>(p.n_blocks) ? 1u : 0u) | (e1 < static_cast<unsigned>(p.n_blocks) ? 2u : 0u);
+            bytes = __popc(valid) * C::GROUP;
             if (win0 + 32 < y1) fetch(win0 + 32);
         };
         auto issue = [&](int stage) {                                    // by the lane that holds the tile
             uint64_t* bar = &bars[warp][stage];
             uint8_t* dst = ring + stage * C::STAGE_BYTES;
-            const uint32_t page_bytes = static_cast<uint32_t>(C::GROUP) << (p.bs_log2 - 4);
-            const uint32_t bytes = __popc(valid) * C::GROUP;
-            auto src = [&](unsigned e) {
-                return p.cache + static_cast<uint64_t>(e * p.H_kv + (f_at >> 4)) * page_bytes + (f_at & 15u) * C::GROUP;
-            };
             s_valid[warp][stage] = valid;
             mbar_arrive_expect_tx(bar, bytes);
             if (!paired) {
-                if (valid) bulk_g2s(dst, src(f0), bytes, bar);           // both groups lie in one page
+                if (valid) bulk_g2s(dst, src0, bytes, bar);              // both groups lie in one page
             } else {
-                if (valid & 1u) bulk_g2s(dst, src(f0), C::GROUP, bar);
-                if (valid & 2u) bulk_g2s(dst + C::GROUP, src(f1), C::GROUP, bar);
+                if (valid & 1u) bulk_g2s(dst, src0, C::GROUP, bar);
+                if (valid & 2u) bulk_g2s(dst + C::GROUP, src1, C::GROUP, bar);
             }
         };
 
