@@ -1,6 +1,6 @@
 // Attention over the 4-bit paged KV cache (include/kf_cache.h) for B200 (sm_100a).
 //
-//   x_j = scale * s_j q . (n_j - z_j),  O = sum_j e^(x_j - m) t_j (n'_j - z'_j) / sum_j e^(x_j - m)
+//   x_j = scale * s_j (q . n_j - z_j sum(q)),  O = sum_j e^(x_j - m) t_j (n'_j - z'_j) / sum_j e^(x_j - m)
 // with (s, z, n) a key's scale, zero point and codes and (t, z', n') a value's.
 //
 // What bounds it: a key and value of one head are D + 8 bytes, read once; at 6.5 TB/s an SM
@@ -9,13 +9,16 @@
 // columns (S^T = K Q^T, O^T = V^T P^T) wastes nothing for up to 8 query rows a cache head; the
 // 128-row tcgen05 tiles would be 1/16 filled and want their operands expanded in memory.
 //
-// Codes to operands.  A 4-bit integer in the low bits of an fp16 is the subnormal n * 2^-24,
-// so `word & 0x000F000F` is a half2 of codes 0 and 4 of eight, `word & 0x00F000F0` of 16 times
-// codes 1 and 5, and a shift by 8 gives the other two.  One half2 FMA (on the FMA pipe, which
-// is idle beside the integer work) makes (n - z) * 2^-9 of each, exact.  Subnormal operands
-// would be exact products too, but the tensor core aligns its sums by the operands' exponent
-// fields and drops their low bits (measured: scores off by 2^-18 instead of 2^-21); and sums of
-// p t (n - z) keep the value's own size, where sum(p t n) - sum(p t z) would cancel.
+// Codes to operands.  A 4-bit integer in bits 2..5 of an fp16 is the subnormal n * 2^-22, in bits
+// 6..9 it is n * 2^-18, and the tensor core multiplies subnormals exactly.  For K two shifts and
+// four ands therefore make four half2 operands of a word's eight codes; the factor 16 goes into the
+// query operand, 2^22 into the score's factor, and the zero point enters once per score.  The
+// tensor core aligns a sum by its operands' exponent fields, which for subnormals are too large by
+// up to 2^8: the low bits this costs leave scores off by 2^-20 (from bits 0..3 and 4..7, with one
+// shift, it was 2^-18; made normal by an FMA each, 2^-21, and 5 % slower).
+// For V two keys' words are interleaved by halves (prmt), masked in place (bits 0..3 and 4..7), and
+// one half2 FMA makes (n - z) * 2^-9 of each pair, exact and normal: sums of p t (n - z) keep the
+// value's own size, where sum(p t n) - sum(p t z) would cancel.
 // Queries are scaled by a power of two per row to a maximum in [2^13, 2^14), which holds fp16
 // rows exactly, and bf16 ones but for elements below 2^-28 of the row's largest.
 // p t enters the second product as fp16, scaled by a power of two such that the largest t seen
@@ -133,7 +136,7 @@ struct Q4Warp {                    // a warp's running state of one unit; pairs:
     float2 m[NT], l[NT];           // reference of the exponent (kQ4NoMax before the first key), sum of p
     float2 mt[NT];                 // this thread's largest score
     uint32_t q[NT][Q4AttnCfg<D, NT>::KW][4];
-    float2 cq[NT];                 // a column's factor of the scores
+    float2 qs[NT], cq[NT];         // -sum(q) * 2^-22, and a column's factor of the scores
     float tmx;                     // this thread's largest value scale
     float tlim, tnorm, tinv;       // value scales up to tlim times tnorm stay below 2^7; tinv = 1 / tnorm
 };
@@ -191,7 +194,7 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
     s.tnorm = s.tinv = 1.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        float x[C::KW][8], mx = 0.f;
+        float x[C::KW][8], mx = 0.f, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < C::KW; ++i) {
             if (p.q_bf16) unpack8<true>(raw[n][i], x[i]);
@@ -207,8 +210,17 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
 #pragma unroll
         for (int i = 0; i < C::KW; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s.q[n][i][e] = pack_half2(x[i][e] * f, x[i][e + 4] * f);
-        const float cq = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(ex - 13) << 23) * 0x1p9f;
+            for (int e = 0; e < 4; ++e) {
+                const float a = x[i][e] * f, b = x[i][e + 4] * f;
+                sum += a + b;
+                s.q[n][i][e] = e & 1 ? pack_half2(a * 0.0625f, b * 0.0625f) : pack_half2(a, b);
+            }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const float qs = sum * -0x1p-22f;
+        const float cq = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(ex - 13) << 23) * 0x1p22f;
+        s.qs[n].x = __shfl_sync(0xffffffffu, qs, 8 * t);
+        s.qs[n].y = __shfl_sync(0xffffffffu, qs, 8 * t + 4);
         s.cq[n].x = __shfl_sync(0xffffffffu, cq, 8 * t);
         s.cq[n].y = __shfl_sync(0xffffffffu, cq, 8 * t + 4);
         s.m[n] = make_float2(kQ4NoMax, kQ4NoMax);
@@ -245,7 +257,6 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
         constexpr int NW = D == 64 ? 2 : 4;
         const uint32_t* words = reinterpret_cast<const uint32_t*>(gr + Q4<D>::K_WORDS);
         const uint32_t wk[2] = {words[g], words[g + 8]};
-        const uint32_t za = q4_negz((wk[0] & 15u) * 0x00010001u), zb = q4_negz((wk[1] & 15u) * 0x00010001u);
 #pragma unroll
         for (int hf = 0; hf < (D == 256 ? 2 : 1); ++hf) {
             uint32_t wa[NW], wb[NW];
@@ -263,9 +274,9 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 const int w = hf * 4 + i;
-                const uint32_t ua = wa[i] >> 8, ub = wb[i] >> 8;
-                const uint32_t a0 = q4_lo(wa[i], za), a1 = q4_lo(wb[i], zb), a2 = q4_hi(wa[i], za), a3 = q4_hi(wb[i], zb);
-                const uint32_t c0 = q4_lo(ua, za), c1 = q4_lo(ub, zb), c2 = q4_hi(ua, za), c3 = q4_hi(ub, zb);
+                const uint32_t ua = wa[i] << 2, ub = wb[i] << 2, va = wa[i] >> 6, vb = wb[i] >> 6;
+                const uint32_t a0 = ua & 0x003C003Cu, a1 = ub & 0x003C003Cu, a2 = ua & 0x03C003C0u, a3 = ub & 0x03C003C0u;
+                const uint32_t c0 = va & 0x003C003Cu, c1 = vb & 0x003C003Cu, c2 = va & 0x03C003C0u, c3 = vb & 0x03C003C0u;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (i == 0) {
@@ -289,12 +300,12 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int key = key0 + 16 * j + 8 * h + g;
-            const float sc = q4_scale(wk[h]);
+            const float sc = q4_scale(wk[h]), z = __uint_as_float(0x4B000000u | (wk[h] & 15u)) - 8388608.0f;
             tv[j][h] = q4_scale(words[16 + g + 8 * h]);
             if (MASKED && (!((valid >> j) & 1u) || key >= len)) tv[j][h] = 0.f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float2 v = fmul2(x[j][n][h], fmul2(make_float2(sc, sc), s.cq[n]));
+                float2 v = fmul2(ffma2(make_float2(z, z), s.qs[n], x[j][n][h]), fmul2(make_float2(sc, sc), s.cq[n]));
                 if (MASKED) {
                     if (!((valid >> j) & 1u)) v = make_float2(0.f, 0.f);     // a page outside the pool reads zeros
                     if (key >= lim[n][0]) v.x = -INFINITY;
@@ -765,7 +776,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                     for (int z = y_cur, sz = stage, pz = phase; z < issued; ++z) {
                         s_drop[warp] = 0;
                         __syncwarp();
-                        mbar_wait_bounded(&bars[warp][sz], pz, &s_drop[warp], p.timeout_ns);
+                        mbar_wait_bounded(&bars[warp][sz], pz, &s_drop[warp], p.timeout_ns + 1000000000ull);
                         __syncwarp();
                         if (++sz == STAGES) { sz = 0; pz ^= 1; }
                     }

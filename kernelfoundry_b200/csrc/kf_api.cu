@@ -1672,7 +1672,7 @@ int kf_attn_fwd_paged_q4(const void* Q, const void* cache, const int* block_tabl
     if (block_size < 16 || block_size > 256 || (block_size & (block_size - 1))) return KF_ERR_INVALID_ARG;
     const long long keys = static_cast<long long>(max_blocks) * block_size;
     const long long R = static_cast<long long>(H_q / H_kv) * S_q;
-    if (keys >= (1ll << 31) || R > kQ4MaxRows || static_cast<long long>(n_blocks) * H_kv >= (1ll << 31))
+    if (keys >= (1ll << 31) - 64 || R > kQ4MaxRows || static_cast<long long>(n_blocks) * H_kv >= (1ll << 31))
         return KF_ERR_INVALID_ARG;
     if (B == 0 || S_q == 0) return KF_OK;
     if (!Q || !cache || !block_table || !seq_lens || !O) return KF_ERR_INVALID_ARG;

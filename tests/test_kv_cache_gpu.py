@@ -295,6 +295,19 @@ def test_mixed_lengths_with_one_dominant(cuda):
     _check(_attn(cuda, q, "f16", cache, table, lens, causal=True), O, A, "f16")
 
 
+@pytest.mark.parametrize("D,H_q,H_kv,n", [(64, 8, 2, 300), (128, 8, 1, 5000), (128, 16, 1, 700), (256, 4, 1, 900)])
+def test_fp32_output_carries_more_than_fp16(cuda, D, H_q, H_kv, n):
+    """With an fp32 output p goes in as two fp16 operands (2^-22 together); what is left are the scores' fp32 errors
+    (absolute, below 2^-17 for these inputs, so as much relative in p) and the sums': 2^-16 A + 2^-24 |O|."""
+    rng = np.random.default_rng(D + n)
+    cache, table = _filled(rng, 1, H_kv, D, 16, [n])
+    q = po.round_to(rng.standard_normal((1, H_q, 1, D)), "f16")
+    O, _, _, A = qo.attention(q, cache, table, [n])
+    got = _host(_attn(cuda, q, "f16", cache, table, [n], out_dtype=_tdt("f32")))
+    tol = 2.0 ** -16 * A + 2.0 ** -24 * np.abs(O)
+    assert (np.abs(got - O) <= tol).all(), f"worst {(np.abs(got - O) / tol).max():.2f}x"
+
+
 def test_scale_growing_maximum_and_outlier_scales(cuda):
     """Scores that rise along the context (the running maximum moves in every tile), values whose scales span 2^40,
     an explicit softmax scale, a negative one."""
