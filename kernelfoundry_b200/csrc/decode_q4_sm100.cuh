@@ -521,6 +521,8 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
 
 // What the merge of a unit across CTAs costs, in tiles of one CTA.
 constexpr unsigned kQ4MergeTiles = 32;
+// What a unit costs a warp besides its tiles (queries in, results out), in tiles.
+constexpr int kQ4UnitTiles = 2;
 
 __device__ __forceinline__ float q4_weight(float m, float M) { return m == -INFINITY ? 0.f : ex2_approx(m - M); }
 
@@ -625,8 +627,10 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     grid_dep_launch_dependents();
     grid_dep_wait();
 
-    // ---- the row of tiles: totals, this CTA's share, this warp's place (every warp for itself:
-    // lane i counts the tiles of sequences i * per ...)
+    // ---- the row of slots: a unit's tiles and kQ4UnitTiles empty slots for what a unit costs by
+    // itself.  Totals, this CTA's share, this warp's place (every warp for itself: lane i counts
+    // sequences i * per ...).
+    constexpr int OV = kQ4UnitTiles;
     const int HR = p.H_kv * p.n_rg;
     const int per = (p.B + 31) >> 5;
     const int b0 = lane * per < p.B ? lane * per : p.B, b1 = b0 + per < p.B ? b0 + per : p.B;
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
 #pragma unroll 4
     for (int b = b0; b < b1; ++b) {
         const int nt = q4_tiles(q4_len(p, b));
-        mine += nt;
+        mine += nt + OV;
         same = same && nt == nt0;
     }
     int incl = mine;
@@ -646,17 +650,17 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         if (lane >= o) incl += v;
     }
     const unsigned T = __shfl_sync(0xffffffffu, incl, 31) * HR;          // < 2^31, the host sees to it
-    // CTAs that take part: every warp of theirs gets at least a tile.  CTA c has the tiles from
-    // c * quot + min(c, rem), warp w of it those from x0 + w * (x1 - x0) / W.
+    // CTAs that take part: every warp of theirs gets at least a slot.  CTA c has the slots from
+    // c * quot + min(c, rem), its warps even shares of them.
     const unsigned want = (T + W - 1) / W;
     unsigned act = want < gridDim.x ? want : gridDim.x, quot = T / act, rem = T - quot * act;
     // Sequences of one length: whole units to each CTA, if that takes no longer than an even
     // split and the merge across CTAs that it needs.
     if (__all_sync(0xffffffffu, same)) {
         const unsigned units = p.B * HR, each = units <= gridDim.x ? 1 : (units + gridDim.x - 1) / gridDim.x;
-        if (each * nt0 <= quot + kQ4MergeTiles) {
+        if (each * (nt0 + OV) <= quot + kQ4MergeTiles) {
             act = each == 1 ? units : (units + each - 1) / each;
-            quot = each * nt0;
+            quot = each * (nt0 + OV);
             rem = 0;
         }
     }
@@ -664,35 +668,42 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
     const int x0 = blockIdx.x * quot + (blockIdx.x < rem ? blockIdx.x : rem);
     const int x1 = blockIdx.x == act - 1 ? T : x0 + quot + (blockIdx.x < rem ? 1 : 0);
     const int wq = (x1 - x0) / W, wr = (x1 - x0) % W;
-    const int y0 = x0 + warp * wq + (warp < wr ? warp : wr), y1 = y0 + wq + (warp < wr ? 1 : 0);
+    const int z0 = x0 + warp * wq + (warp < wr ? warp : wr), z1 = z0 + wq + (warp < wr ? 1 : 0);
+
+    // The tile at slot z (of an empty slot: the next unit's first) and its number among all tiles.
+    auto locate = [&](int z, Q4Cursor& c) {
+        const int lo = (incl - mine) * HR;
+        const bool here = z >= lo && z < incl * HR;
+        int b = b0, at = lo;
+        if (here)
+            for (; b < b1 - 1; ++b) {
+                const int next = at + (q4_tiles(q4_len(p, b)) + OV) * HR;
+                if (z < next) break;
+                at = next;
+            }
+        const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+        c.b = __shfl_sync(0xffffffffu, b, from);
+        at = __shfl_sync(0xffffffffu, at, from);
+        c.len = q4_len(p, c.b);
+        c.nt = q4_tiles(c.len);
+        const unsigned off = z - at, hr = off / (c.nt + OV), o = off - hr * (c.nt + OV);
+        c.tile = static_cast<int>(o) < c.nt ? o : c.nt;
+        c.h = hr;
+        c.rg = 0;
+        if (p.n_rg > 1) {
+            c.h = hr / p.n_rg;
+            c.rg = hr - c.h * p.n_rg;
+        }
+        const int y = at - OV * HR * c.b + hr * c.nt + c.tile;
+        if (c.tile == c.nt) q4_next_unit(p, c);
+        return y;
+    };
+    Q4Cursor cur, next;
+    const int y0 = z0 < z1 ? locate(z0, cur) : 0;
+    const int y1 = z0 == z1 ? 0 : z1 == static_cast<int>(T) ? z1 - OV * HR * p.B : locate(z1, next);
 
     if (y0 < y1) {
         int y_cur = y0;                                                  // the tile in work
-        Q4Cursor cur;
-        {
-            const int lo = (incl - mine) * HR;
-            const bool here = y0 >= lo && y0 < incl * HR;
-            int b = b0, at = lo;
-            if (here)
-                for (; b < b1 - 1; ++b) {
-                    const int next = at + q4_tiles(q4_len(p, b)) * HR;
-                    if (y0 < next) break;
-                    at = next;
-                }
-            const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-            cur.b = __shfl_sync(0xffffffffu, b, from);
-            const unsigned off = y0 - __shfl_sync(0xffffffffu, at, from);
-            cur.len = q4_len(p, cur.b);
-            cur.nt = q4_tiles(cur.len);
-            const unsigned hr = off / cur.nt;
-            cur.tile = off - hr * cur.nt;
-            cur.h = hr;
-            cur.rg = 0;
-            if (p.n_rg > 1) {
-                cur.h = hr / p.n_rg;
-                cur.rg = hr - cur.h * p.n_rg;
-            }
-        }
         uint4 raw[NT][C::KW];
         q4_load_q<D, NT>(p, raw, cur, lane);                             // ahead of the copies
 
@@ -840,8 +851,9 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
             return reinterpret_cast<const float*>(f & 1 ? smem + (f >> 1) * (STAGES * C::STAGE_BYTES)
                                                         : smem + C::RING_BYTES + (f >> 1) * (C::PART_FLOATS * 4));
         };
-        const bool inside = us >= x0 && us + unt <= x1;
-        const int slot = us >= x0 ? 1 : 0;
+        const int ws = us + OV * u;                                      // the unit's first slot
+        const bool inside = ws >= x0 && ws + unt <= x1;
+        const int slot = ws >= x0 ? 1 : 0;
         float* out = p.parts + (static_cast<size_t>(blockIdx.x) * 2 + slot) * C::PART_FLOATS;
         const bool ours = teams == 1 || run_no % teams == team;
         ++run_no;
@@ -866,7 +878,7 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
                 const unsigned big = rem * (quot + 1);
                 return static_cast<int>(x < big ? x / (quot + 1) : rem + (x - big) / quot);
             };
-            const int cf = slot ? static_cast<int>(blockIdx.x) : cta_of(us), cl = cta_of(us + unt - 1);
+            const int cf = slot ? static_cast<int>(blockIdx.x) : cta_of(ws), cl = cta_of(ws + unt - 1);
 #pragma unroll
             for (int k = 0; k < 2; ++k)
                 if (k == slot) {

@@ -1679,7 +1679,7 @@ int kf_attn_fwd_paged_q4(const void* Q, const void* cache, const int* block_tabl
     if (!aligned16(Q) || !aligned16(cache) || !aligned16(O) || !aligned16(workspace)) return KF_ERR_MISALIGNED;
     const int nt = q4_attn_nt(D, static_cast<int>(R));
     const int n_rg = static_cast<int>((R + 8 * nt - 1) / (8 * nt));
-    const long long tiles = static_cast<long long>(B) * H_kv * n_rg * ((keys + 31) / 32);   // an upper bound
+    const long long tiles = static_cast<long long>(B) * H_kv * n_rg * ((keys + 31) / 32 + kf::kQ4UnitTiles);   // an upper bound
     if (tiles >= (1ll << 31)) return KF_ERR_INVALID_ARG;
     DeviceInfo* di = nullptr;
     int rc = device_info(&di);
