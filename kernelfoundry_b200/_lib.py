@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+
 from .build import LIB_PATH
 
 KF_OK = 0
@@ -186,8 +188,6 @@ def on_device(index: int, fn, what: str, *args) -> None:
     The two torch calls are the ones behind torch.cuda.current_stream / current_device, without
     the Stream object and the lazy-initialisation check (a tensor on the device exists): the
     small operators' host cost is mostly this."""
-    import torch
-
     if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:

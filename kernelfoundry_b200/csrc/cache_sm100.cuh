@@ -27,44 +27,46 @@ constexpr uint32_t kQ4BadRow = 0x7FC00000u;                 // word of a row wit
 __device__ __forceinline__ float q4_scale(uint32_t w) { return __uint_as_float(w & 0xFFFFFF00u); }
 
 // Parameter word of a row from its extremes (lo <= 0 <= hi, NaN if the row has one) and what
-// the codes need: the reciprocal scale and the zero point (both 0 for a spoiled row).
-__device__ __forceinline__ uint32_t q4_params(float lo, float hi, float* inv, float* zp) {
+// the codes need: the reciprocal scale (0 for a spoiled row); its low bits are the zero point.
+__device__ __forceinline__ uint32_t q4_params(float lo, float hi, float* inv) {
     const float c = 1.0f / 15.0f;
     float s = __fsub_rn(__fmul_rn(hi, c), __fmul_rn(lo, c));
     if (!(fabsf(s) <= 3.402823466e38f)) {                   // finite exactly when the row is
-        *inv = *zp = 0.0f;
+        *inv = 0.0f;
         return kQ4BadRow;
     }
     s = __uint_as_float((__float_as_uint(s) + 0x80u) & 0xFFFFFF00u);
     if (s < 7.888609052210118e-31f) s = 0.0f;               // 2^-100: keeps 1/s finite
     *inv = s == 0.0f ? 0.0f : __frcp_rn(s);
-    *zp = fminf(fmaxf(rintf(__fmul_rn(-lo, *inv)), 0.0f), 15.0f);
-    return __float_as_uint(s) | static_cast<uint32_t>(*zp);
+    return __float_as_uint(s) | static_cast<uint32_t>(rintf(__fmul_rn(-lo, *inv)));
 }
 
 // Eight codes, clamp(rint(x * inv) + zp, 0, 15), in a word.  Adding 1.5 * 2^23 rounds to an integer
-// (ties to even); the clamp is taken around it, and the nibbles are put together by exact FMAs.
-__device__ __forceinline__ uint32_t q4_codes8(const float (&x)[8], float inv, float zp) {
-    const float m = 12582912.0f, lo = m - zp, hi = lo + 15.0f;
-    float n[8];
+// r (ties to even) and leaves it as 0x4B400000 + r, so the sum of these words times 16^e, less the
+// constants', is the sum of r 16^e; zp goes in eight times at once.  The lower clamp never acts:
+// rint(x inv) >= rint(lo inv) = -zp, and zp needs none, as s >= (hi - lo) / 15 * (1 - 2^-16).
+__device__ __forceinline__ uint32_t q4_codes8(const float (&x)[8], float inv, uint32_t zp) {
+    const float top = 12582912.0f + static_cast<float>(15 - static_cast<int>(zp));
+    uint32_t w = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-        // (not packed: a packed product and sum of explicit rounding were still fused into one FMA)
-        const float q0 = __fadd_rn(__fmul_rn(x[e], inv), m), q1 = __fadd_rn(__fmul_rn(x[e + 1], inv), m);
-        const float2 y = fadd2(make_float2(fminf(fmaxf(q0, lo), hi), fminf(fmaxf(q1, lo), hi)), make_float2(-lo, -lo));
-        n[e] = y.x;
-        n[e + 1] = y.y;
-    }
-    float h[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        h[i] = fmaf(fmaf(n[4 * i + 3], 16.0f, n[4 * i + 2]), 256.0f, fmaf(n[4 * i + 1], 16.0f, n[4 * i]));
-    return __float2uint_rz(h[0]) | __float2uint_rz(h[1]) << 16;
+    for (int e = 7; e >= 0; --e)        // (not packed: a packed product and sum, both rounded, were still fused into an FMA)
+        w = w * 16u + __float_as_uint(fminf(__fadd_rn(__fmul_rn(x[e], inv), 12582912.0f), top));
+    return w + zp * 0x11111111u - 0x4B400000u * 0x11111111u;
 }
 
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+// Larger of two packed pairs, NaN if either is.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
 
@@ -121,26 +123,29 @@ __device__ __forceinline__ uint8_t* q4_group(const Q4IoParams& p, int slot, int 
     return p.cache + static_cast<unsigned long long>(((block * p.H + h) << gs) + ((slot >> 4) & ((1u << gs) - 1))) * Q4<D>::GROUP;
 }
 
-// A row belongs to D / 16 threads with the vectors u and u + D / 16: a store of their words is a
-// whole sector.
+// A row belongs to D / 32 threads with four neighbouring vectors each: their words are one 16-byte
+// store, and the row's parameters are worked out by few threads.  The extremes are found on packed
+// pairs, the largest value and the largest negated one in the halves of one word.  (Two vectors a
+// thread and fp32 extremes: 87 us for 65536 tokens, at 15 instructions an element.)
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256, 3) q4_write_kernel(const Q4IoParams p) {
-    constexpr int GS = D / 16, RG = 256 / GS, UNR = 4;
+    constexpr int GS = D / 32, RG = 256 / GS, UNR = 2;
     const int u = threadIdx.x % GS;
     const unsigned row0 = blockIdx.x * (p.passes * RG) + threadIdx.x / GS;
-    uint4 x4[UNR][2];
+    uint4 x4[UNR][4];
     int slot[UNR], h[UNR];                                           // head; V's have bit 30 set
 #pragma unroll
     for (int i = 0; i < UNR; ++i) {
         const unsigned row = row0 + i * RG;
         slot[i] = -1;
         h[i] = 0;
-        x4[i][0] = x4[i][1] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x4[i][c] = make_uint4(0u, 0u, 0u, 0u);
         if (i < p.passes && row < p.rows) {
             const Q4Row r = q4_row(p, row);
-            const uint4* src = (r.is_v ? p.v : p.k) + r.at;
-            x4[i][0] = ld_stream(src + u);
-            x4[i][1] = ld_stream(src + u + GS);
+            const uint4* src = (r.is_v ? p.v : p.k) + r.at + 4 * u;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x4[i][c] = src[c];
             slot[i] = p.slots[r.tok];
             h[i] = r.is_v ? r.h | 1 << 30 : r.h;
         }
@@ -148,34 +153,36 @@ __global__ void __launch_bounds__(256, 3) q4_write_kernel(const Q4IoParams p) {
 #pragma unroll
     for (int i = 0; i < UNR; ++i) {
         if (i >= p.passes) break;
-        float x[2][8], lo = 0.f, hi = 0.f;
+        uint32_t mx = 0u, mn = 0u;                                   // (0 is always within the row's range)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            unpack8<BF16>(x4[i][c], x[c]);
+        for (int c = 0; c < 4; ++c) {
+            const uint32_t w[4] = {x4[i][c].x, x4[i][c].y, x4[i][c].z, x4[i][c].w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                lo = fminf(lo, x[c][e]);
-                hi = fmax_nan(hi, x[c][e]);
+            for (int e = 0; e < 4; ++e) {
+                mx = max2_nan<BF16>(mx, w[e]);
+                mn = min2_nan<BF16>(mn, w[e]);
             }
         }
+        mn ^= 0x80008000u;
+        uint32_t ext = max2_nan<BF16>(__byte_perm(mx, mn, 0x5410), __byte_perm(mx, mn, 0x7632));
 #pragma unroll
-        for (int o = GS / 2; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmax_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
+        for (int o = GS / 2; o > 0; o >>= 1) ext = max2_nan<BF16>(ext, __shfl_xor_sync(0xffffffffu, ext, o));
         const bool is_v = h[i] >> 30;
         uint8_t* g = q4_group<D>(p, slot[i], h[i] & 0xFFFF);
         if (!g) continue;
-        float inv, zp;
-        const uint32_t word = q4_params(lo, hi, &inv, &zp);
+        float inv;
+        const uint32_t word = q4_params(-to_f32<BF16>(ext >> 16), to_f32<BF16>(ext & 0xFFFFu), &inv);
         const int rr = slot[i] & 15;
-        uint32_t* w = reinterpret_cast<uint32_t*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW);
-        if (word == kQ4BadRow) {
-            w[u] = w[u + GS] = 0u;
-        } else {
-            w[u] = q4_codes8(x[0], inv, zp);
-            w[u + GS] = q4_codes8(x[1], inv, zp);
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (word != kQ4BadRow) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float x[8];
+                unpack8<BF16>(x4[i][c], x);
+                w[c] = q4_codes8(x, inv, word & 15u);
+            }
         }
+        reinterpret_cast<uint4*>(g + (is_v ? Q4<D>::V_CODES : 0) + rr * Q4<D>::ROW)[u] = make_uint4(w[0], w[1], w[2], w[3]);
         if (u == 0) reinterpret_cast<uint32_t*>(g + (is_v ? Q4<D>::V_WORDS : Q4<D>::K_WORDS))[rr] = word;
     }
 }

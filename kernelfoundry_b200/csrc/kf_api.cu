@@ -1613,8 +1613,9 @@ int q4_io_launch(kf::Q4IoParams p, bool write, cudaStream_t s) {
     DeviceInfo* di = nullptr;
     const int rc = device_info(&di);
     if (rc != KF_OK) return rc;
-    const long long pass = 4096 / D;                      // rows of a block's pass
-    p.passes = p.rows >= 4 * pass * 4 * di->sm_count ? 4 : 1;
+    const long long pass = (write ? 8192 : 4096) / D;     // rows of a block's pass
+    const int most = write ? 2 : 4;
+    p.passes = p.rows >= most * pass * 4 * di->sm_count ? most : 1;
     const unsigned grid = static_cast<unsigned>((p.rows + p.passes * pass - 1) / (p.passes * pass));
     if (write) kf::q4_write_kernel<D, BF16><<<grid, 256, 0, s>>>(p);
     else kf::q4_read_kernel<D, BF16><<<grid, 256, 0, s>>>(p);

@@ -147,8 +147,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
         out = (torch.empty_like(q, memory_format=torch.contiguous_format),
                torch.empty_like(k, memory_format=torch.contiguous_format) if k is not None else None)
     q_out, k_out = out
-    key = (layout, interleaved, rot_dim, *(None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-                                           for t in (q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq)))
+    key = (layout, interleaved, rot_dim, q.shape, q.stride(), q.dtype, q.device, q_out.shape, q_out.stride(), q_out.dtype,
+           q_out.device, _form(k), _form(k_out), _form(q_weight), _form(k_weight), _form(positions), _form(inv_freq))
     plan = _qk_plans.get(key) or _qk_plans.put(key, _plan_qk_norm_rope(
         q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq, layout, interleaved, rot_dim))
     index, (B, S, H_q, H_kv, D, rot), (_, strides), flags = plan
@@ -161,6 +161,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
 
 
 _qk_plans = CallPlans()
+
+
+def _form(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 def _plan_qk_norm_rope(q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq, layout, interleaved, rot_dim):
