@@ -1418,7 +1418,7 @@ int kf_rope(void* q, void* k, const int* positions, const float* inv_freq, int B
     int hg_target = 64 / p.U;
     if (hg_target < 1) hg_target = 1;
     const int need = (H + hg_target - 1) / hg_target;
-    const int hb = need <= 1 ? 1 : need <= 4 ? 4 : 2;
+    const int hb = need <= 1 ? 1 : need <= 4 ? 4 : 8;
     p.HG = (H + hb - 1) / hb;
     p.TPB = 256 / (p.U * p.HG);
     if (p.TPB < 1) p.TPB = 1;
