@@ -12,7 +12,6 @@
 
 namespace kf {
 
-constexpr int kQ4GroupTokens = 16;
 template <int D>
 struct Q4 {
     static constexpr int ROW = D / 2;                       // bytes of one row of codes
@@ -209,6 +208,8 @@ __device__ __forceinline__ void q4_values8(uint32_t w, const float (&zc)[5], con
 }
 
 // A row belongs to D / 16 threads with the words (8 codes, one 16-byte vector) u and u + D / 16.
+// 65536 tokens of 8 heads of 128: 57.1 us, 5.95 TB/s of results and codes (write: 61.7 us, 5.5 TB/s); a long
+// read is bound by its writes to memory, 8192 tokens (9.7 us) by instructions and by starting and draining.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256, 4) q4_read_kernel(const Q4IoParams p) {
     constexpr int GS = D / 16, RG = 256 / GS, UNR = 4;

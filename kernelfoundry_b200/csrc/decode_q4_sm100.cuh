@@ -30,7 +30,7 @@
 // instead of a maximum across the warp.  The true maximum is kept per thread and put in at the end.
 //
 // Work split.  Every (sequence, cache head, group of 8 NT query rows) is a unit of 32-key
-// tiles; all units' tiles in a row are cut evenly over the CTAs (one per SM) and each CTA's
+// tiles; all units' tiles in a row (and kQ4UnitTiles more for each unit) are cut evenly over the CTAs (one per SM) and each CTA's
 // share over its warps.  A warp is on its own: it copies its tiles (cp.async.bulk, one or two
 // 16-token groups each) into its ring, waits, computes and refills, with no CTA barrier, and
 // carries (m, l, O) in registers.  Lengths are read on the device, so the split is even
@@ -38,6 +38,12 @@
 // at the CTA's end in shared memory, and units that cross CTAs by the last CTA to arrive
 // (at most two parts per CTA in the workspace, merged in CTA order: results do not depend on
 // timing).
+//
+// Measured, 32 query and 8 cache heads of 128 (bytes of codes and words over time; 6.55 TB/s is a copy):
+// B=64, KV=4096 66.5 us (4.3 TB/s), B=16 25.2 (2.8), B=1, KV=131072 38.4 (3.7), B=1, KV=512 8.0.  The copies
+// alone take 46 us at B=64 and 24.6 at KV=131072; the rest is instructions (293 for 16 keys, at 2.2
+// to 2.4 a clock, the ALU pipe busiest) and, for few sequences, the chain of loads before the first
+// tile (about 6000 clocks) and the merges.
 #pragma once
 
 #include "cache_sm100.cuh"
@@ -66,8 +72,11 @@ struct Q4AttnParams {
 template <int D_, int NT_>
 struct Q4AttnCfg {
     static constexpr int D = D_, NT = NT_;
+    // As many warps as the registers allow without spills (D = 64 with 12 warps: 51.2 us instead of 45.8 at
+    // B=32, KV=8192; D = 128 with 16: 128 registers, which spill).  Two stages hide the copies; a third
+    // costs 0 to 2 % at 12 warps of 8 rows and gains 2 % at 8 warps of 16.
     static constexpr int W = D == 256 ? 8 : NT == 1 ? (D == 64 ? 16 : 12) : (D == 64 ? 12 : 8);   // warps
-    static constexpr int STAGES = D == 256 ? 2 : D == 64 ? 4 : NT == 1 ? 2 : 4;
+    static constexpr int STAGES = NT == 2 || D == 64 ? 3 : 2;
     static constexpr int THREADS = 32 * W;
     static constexpr int GROUP = Q4<D>::GROUP;
     static constexpr int STAGE_BYTES = 2 * GROUP;                // a tile: 32 keys
@@ -519,9 +528,11 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
     }
 }
 
-// What the merge of a unit across CTAs costs, in tiles of one CTA.
+// What the merge of a unit across CTAs costs, in tiles of one CTA.  (With 0, an even split whenever it is
+// shorter: B=1, KV=512 9.0 us instead of 8.0, B=16, KV=4096 25.7 instead of 25.2.)
 constexpr unsigned kQ4MergeTiles = 32;
-// What a unit costs a warp besides its tiles (queries in, results out), in tiles.
+// What a unit costs a warp besides its tiles (queries in, results out), in tiles.  (With 0: 48 sequences
+// of 1 to 8192 keys 24.6 us instead of 18.2.)
 constexpr int kQ4UnitTiles = 2;
 
 __device__ __forceinline__ float q4_weight(float m, float M) { return m == -INFINITY ? 0.f : ex2_approx(m - M); }

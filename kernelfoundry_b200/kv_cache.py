@@ -20,6 +20,7 @@ from ._lib import (KF_CACHE_BF16, KF_FLAG_CAUSAL, KF_FLAG_OUT_BF16, KF_FLAG_OUT_
 __all__ = ["q4_cache", "kv_write_q4", "kv_read_q4", "flash_attn_paged_q4"]
 
 _ws: dict[tuple[int, int], torch.Tensor] = {}    # (device, stream) -> zero-filled workspace, grown on demand
+_ws_outgrown: list[torch.Tensor] = []            # kept (a few MB at most): a captured graph may hold their addresses
 
 _IO_FLAGS = {torch.float16: 0, torch.bfloat16: KF_CACHE_BF16}
 _OUT_FLAGS = {torch.float32: 0, torch.float16: KF_FLAG_OUT_F16, torch.bfloat16: KF_FLAG_OUT_BF16}
@@ -71,6 +72,8 @@ def _workspace(device, nbytes):
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
         if not torch.cuda.is_current_stream_capturing():   # memory of a graph's pool stays with the graph
+            if key in _ws:
+                _ws_outgrown.append(_ws[key])
             _ws[key] = ws
     return ws
 

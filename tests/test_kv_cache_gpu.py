@@ -430,6 +430,39 @@ def test_repeatable_streams_graphs_and_shared_workspace(cuda):
     assert device_error()[0] == 0
 
 
+def test_graph_keeps_its_streams_workspace(cuda):
+    """A graph captured with the stream's own workspace stays right after calls that need a larger one and new tensors
+    that could have taken its place."""
+    import torch
+
+    from kernelfoundry_b200 import flash_attn_paged_q4
+
+    rng = np.random.default_rng(23)
+    to = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)  # noqa: E731
+    inputs = []
+    for D, H_q in ((64, 4), (128, 32), (256, 4)):
+        cache, table = _filled(rng, 2, 2, D, 16, [700, 90], poison=False)
+        t = to(table).clamp_(0, cache.shape[0] - 1)
+        inputs.append((_dev(rng.standard_normal((2, H_q, 1, D)), "f16", cuda), to(cache), t, to(np.array([700, 90], np.int32))))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = flash_attn_paged_q4(*inputs[0])
+        out = torch.empty_like(want)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            flash_attn_paged_q4(*inputs[0], out=out)
+        others = [flash_attn_paged_q4(*x) for x in inputs[1:]]
+        junk = [torch.full((n,), 255, dtype=torch.uint8, device=cuda) for n in (1 << 19, 1 << 20, 1 << 21, 1 << 21)]
+        graph.replay()
+        stream.synchronize()
+        assert torch.equal(out, want)
+        assert all(bool((j == 255).all()) for j in junk)
+        assert all(torch.equal(flash_attn_paged_q4(*x), y) for x, y in zip(inputs[1:], others))
+        stream.synchronize()
+
+
 def test_written_cache_attends_like_its_read_back_values(cuda):
     """write -> attend equals read back -> flash_attn_fwd within both calls' rounding (K, V rounded to fp16 on read)."""
     import torch
