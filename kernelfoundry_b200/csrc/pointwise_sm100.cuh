@@ -326,31 +326,51 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const QkNormRopePa
     // Pairs 2e, 2e + 1 of thread u, token t, queries (0) or keys (1): (A, A', B, B') and (C, C', S, S')
     // at [kind][t][2e, 2e + 1][u]:  y0 = x0 A + x1 B,  y1 = x1 C + x0 S.
     __shared__ float4 s_c[2 * kQkNormRopePairs];
+    // Pair j = eU + u of a row: half turns per position, and the weights (w0, w1) for queries and keys.
     __shared__ double s_f[256];
-    // q, k, q_out, k_out offsets and position of each token, of this group and of the next
-    __shared__ unsigned long long s_off[2][4][kQkNormRopeTokens];
+    __shared__ float4 s_w[256];
+    // 16-byte indices of a token's first input and output vector, [token][queries or keys], and its
+    // position, of this group and of the next
+    __shared__ ulonglong2 s_at[2][2 * kQkNormRopeTokens];
     __shared__ int s_pos[2][kQkNormRopeTokens];
     const int tid = threadIdx.x, half = p.rot_dim >> 1, H = p.H_q + p.H_kv;
     auto tokens = [&](int item, int buf) {
         const unsigned t = (item / p.splits) * p.TPB + tid;
         if (tid >= p.TPB || t >= p.n_tokens) return;
         const unsigned b = t / p.S, s = t - b * p.S;
-        auto at = [&](unsigned sb, unsigned ss) { return static_cast<unsigned long long>(b) * sb + static_cast<unsigned long long>(s) * ss; };
-        s_off[buf][0][tid] = at(p.q_sb, p.q_ss);
-        s_off[buf][1][tid] = at(p.k_sb, p.k_ss);
-        s_off[buf][2][tid] = at(p.qo_sb, p.qo_ss);
-        s_off[buf][3][tid] = at(p.ko_sb, p.ko_ss);
+        auto at = [&](const uint4* x, unsigned sb, unsigned ss) {
+            return (reinterpret_cast<unsigned long long>(x) >> 4) + static_cast<unsigned long long>(b) * sb +
+                   static_cast<unsigned long long>(s) * ss;
+        };
+        s_at[buf][2 * tid] = make_ulonglong2(at(p.q, p.q_sb, p.q_ss), at(p.qo, p.qo_sb, p.qo_ss));
+        s_at[buf][2 * tid + 1] = make_ulonglong2(at(p.k, p.k_sb, p.k_ss), at(p.ko, p.ko_sb, p.ko_ss));
         s_pos[buf][tid] = p.pos ? p.pos[t] : static_cast<int>(s);
     };
     tokens(blockIdx.x, 0);
-    for (int i = tid; i < half; i += 256)
-        s_f[i] = 0.3183098861837907 *                      // half turns per position
-                 (p.inv_freq ? static_cast<double>(p.inv_freq[i]) : exp2(-(2.0 * i / p.rot_dim) * p.log2_theta));
+    const int U = p.D >> 4, r = p.rot_dim >> 4;            // threads of a row that hold something; that rotate (NeoX)
+    // The pair whose coefficients this thread makes, of tokens ct, ct + ct_step, ...
+    const int ct = tid / (8 * U), ct_step = 256 / (8 * U), cj = tid - ct * 8 * U, ce = cj / U, cu = cj - ce * U;
+    int i0, i1, pr;
+    if (NEOX) {
+        i0 = cu < r ? 8 * cu + ce : 16 * cu + ce;
+        i1 = cu < r ? i0 + half : i0 + 8;
+        pr = cu < r ? i0 : -1;
+    } else {
+        i0 = 8 * (ce < 4 ? cu : cu + U) + 2 * (ce & 3);
+        i1 = i0 + 1;
+        pr = i0 < p.rot_dim ? i0 >> 1 : -1;
+    }
+    const bool rotates = pr >= 0;
+    if (ct == 0) {
+        auto weight = [](const uint4* w, int i) { return w ? to_f32<BF16>(reinterpret_cast<const uint16_t*>(w)[i]) : 1.f; };
+        s_w[cj] = make_float4(weight(p.qw, i0), weight(p.qw, i1), weight(p.kw, i0), weight(p.kw, i1));
+        s_f[cj] = !rotates ? 0.0 : 0.3183098861837907 *
+                  (p.inv_freq ? static_cast<double>(p.inv_freq[pr]) : exp2(-(2.0 * pr / p.rot_dim) * p.log2_theta));
+    }
     __syncthreads();
 
-    // row groups, this thread's, its place in the row, threads of a row that hold something
-    const int RG = 256 / p.GS, rg = tid / p.GS, u = tid & (p.GS - 1), U = p.D >> 4;
-    const int r = p.rot_dim >> 4;
+    // row groups, this thread's, its place in the row; tokens and heads from one of its rows to the next
+    const int RG = 256 / p.GS, rg = tid / p.GS, u = tid & (p.GS - 1), dt = RG / H, dh = RG - dt * H;
     const int c0 = !NEOX || u < r ? u : 2 * u, c1 = !NEOX ? u + U : u < r ? u + r : 2 * u + 1;   // its vectors
     const bool on = u < U;
 
@@ -373,42 +393,38 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const QkNormRopePa
                 if (row + i * RG < end && on) {
                     const bool is_q = h < p.H_q;
                     const unsigned hh = is_q ? h : h - p.H_q;
-                    const uint4* src = (is_q ? p.q : p.k) + s_off[buf][is_q ? 0 : 1][tk] +
-                                       static_cast<unsigned long long>(hh) * (is_q ? p.q_sh : p.k_sh);
-                    out[i] = (is_q ? p.qo : p.ko) + s_off[buf][is_q ? 2 : 3][tk] +
-                             static_cast<unsigned long long>(hh) * (is_q ? p.qo_sh : p.ko_sh);
+                    const ulonglong2 base = s_at[buf][2 * tk + (is_q ? 0 : 1)];
+                    const uint4* src = reinterpret_cast<const uint4*>(
+                        (base.x + static_cast<unsigned long long>(hh) * (is_q ? p.q_sh : p.k_sh)) << 4);
+                    out[i] = reinterpret_cast<uint4*>(
+                        (base.y + static_cast<unsigned long long>(hh) * (is_q ? p.qo_sh : p.ko_sh)) << 4);
                     at[i] = ((is_q ? 0 : n_tok) + tk) * 8 * U + u;
                     v[i][0] = ld_stream(src + c0);
                     v[i][1] = ld_stream(src + c1);
                 }
-                for (h += RG; h >= H; h -= H) ++tk;
+                h += dh;
+                tk += dt;
+                if (h >= H) {
+                    h -= H;
+                    ++tk;
+                }
             }
             if (first) {                                                     // while the first rows are on their way
                 first = false;
-                for (int i = tid; i < n_tok * 8 * U; i += 256) {
-                    const int t = i / (8 * U), e = (i - t * 8 * U) / U, w = i - t * 8 * U - e * U;   // pair e of thread w
-                    int i0, i1, pr;
-                    if (NEOX) {
-                        i0 = w < r ? 8 * w + e : 16 * w + e;
-                        i1 = w < r ? i0 + half : i0 + 8;
-                        pr = w < r ? i0 : -1;
-                    } else {
-                        i0 = 8 * (e < 4 ? w : w + U) + 2 * (e & 3);
-                        i1 = i0 + 1;
-                        pr = i0 < p.rot_dim ? i0 >> 1 : -1;
-                    }
+                const float4 wt = s_w[cj];
+                const double f = s_f[cj];
+                for (int t = ct < ct_step ? ct : n_tok; t < n_tok; t += ct_step) {
                     float sn = 0.f, cs = 1.f;
-                    if (pr >= 0) {
-                        const double a = s_pos[buf][t] * s_f[pr];
+                    if (rotates) {
+                        const double a = s_pos[buf][t] * f;
                         sincospif(static_cast<float>(a - 2.0 * rint(0.5 * a)), &sn, &cs);
                         sn *= p.rot_scale;
                         cs *= p.rot_scale;
                     }
 #pragma unroll
                     for (int kind = 0; kind < 2; ++kind) {
-                        const uint16_t* wt = reinterpret_cast<const uint16_t*>(kind ? p.kw : p.qw);
-                        const float w0 = wt ? to_f32<BF16>(wt[i0]) : 1.f, w1 = wt ? to_f32<BF16>(wt[i1]) : 1.f;
-                        float* c = reinterpret_cast<float*>(s_c + ((kind * n_tok + t) * 8 + (e & ~1)) * U + w) + (e & 1);
+                        const float w0 = kind ? wt.z : wt.x, w1 = kind ? wt.w : wt.y;
+                        float* c = reinterpret_cast<float*>(s_c + ((kind * n_tok + t) * 8 + (ce & ~1)) * U + cu) + (ce & 1);
                         c[0] = w0 * cs;
                         c[2] = -w1 * sn;
                         c[4 * U] = w1 * cs;
