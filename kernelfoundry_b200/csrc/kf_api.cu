@@ -1480,8 +1480,9 @@ int kf_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
     p.rot_dim = rot_dim;
     p.GS = 1;
     while (p.GS < D / 16) p.GS <<= 1;
-    // Groups of tokens: as large as leave two an SM (2331 tokens of 15 heads of 256: 4 a group 11.0 us,
-    // 8 13.0, 1 24); where there are fewer tokens than that the rows of a token are split.
+    // Groups of tokens: as large as leave two an SM (8192 tokens of 40 heads of 128: 8 a group 33.4 us, 4 34.3,
+    // 2 38.9; 2331 of 15 of 256: 4 a group 9.9, 2 10.8); where there are fewer tokens than that the rows of a
+    // token are split.
     const int H = H_q + H_kv, rows_at_once = 256 / p.GS, sms = di->sm_count;
     p.TPB = kf::kQkNormRopeTokens;
     while (p.TPB > 1 && (p.TPB * (D / 2) > kf::kQkNormRopePairs || n_tokens < 2ll * sms * p.TPB)) p.TPB >>= 1;

@@ -291,8 +291,9 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 // takes groups of whole tokens: while a group's first rows are on their way it computes each pair's four
 // coefficients (cos and sin times both weights, for queries and for keys; angles in half turns,
 // reduced in fp64) into shared memory, and a row then costs one scaling and four packed FMAs a
-// pair.  (Weights in registers and cos / sin alone in the table took 23 instructions an element,
-// 46.5 us for 8192 tokens of 40 heads of 128, against 25.6 us for the bytes.)  A row belongs to
+// pair.  8192 tokens of 40 heads of 128 take 33.4 us (5.0 TB/s; 25.6 us are the bytes), at 14.5 instructions
+// an element and 2.5 a clock.  (Weights in registers and cos / sin alone in the table took 23
+// instructions, 46.5 us.)  A row belongs to
 // GS = 2^k >= D / 16 threads with two 8-element vectors each, paired so that both halves of a NeoX
 // rotation are in one thread: vectors (u, u + rot_dim / 16) rotate, the rest pass through as
 // pairs with cos = 1; the sum of squares is reduced by shuffles.
@@ -322,7 +323,7 @@ constexpr int kQkNormRopePairs = 1024;                     // TPB * D / 2 at mos
 
 template <bool BF16, bool NEOX>
 __global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const QkNormRopeParams p) {
-    constexpr int UNR = 2;                                 // rows a thread has in flight (4: fewer warps fit, 40 us)
+    constexpr int UNR = 2;                                 // rows a thread has in flight (1: 37.2 us; 3, in three blocks an SM: 37.0)
     // Pairs 2e, 2e + 1 of thread u, token t, queries (0) or keys (1): (A, A', B, B') and (C, C', S, S')
     // at [kind][t][2e, 2e + 1][u]:  y0 = x0 A + x1 B,  y1 = x1 C + x0 S.
     __shared__ float4 s_c[2 * kQkNormRopePairs];
