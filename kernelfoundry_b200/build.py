@@ -1,22 +1,27 @@
-"""Build libkf_attn.so (sm_100a only) in-tree.
+"""Build libkf_attn.so (sm_100a only) and _kf_host.so in-tree.
 
     python -m kernelfoundry_b200.build [--verbose]
 
 nvcc cross-compiles for B200 without a GPU.  The library links the static CUDA
 runtime and reaches the driver only through cudaGetDriverEntryPoint, so it
-loads (and its argument checks run) on machines without a GPU driver.
+loads (and its argument checks run) on machines without a GPU driver.  _kf_host.so is the
+host side of the small operators' Python calls (csrc/kf_host.cpp), built against the installed
+torch.
 """
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.environ.get("KF_LIB_PATH") or os.path.join(LIB_DIR, "libkf_attn.so")
+HOST_PATH = os.path.join(LIB_DIR, "_kf_host.so")
+HOST_SOURCE = os.path.join(CSRC, "kf_host.cpp")
 SOURCES = ["kf_api.cu"]
 HEADERS = ["kf_ptx.cuh", "prefill_sm100.cuh", "decode_sm100.cuh", "pointwise_sm100.cuh", "peer_sm100.cuh",
            "synth_sm100.cuh", "cache_sm100.cuh", "decode_q4_sm100.cuh"]
@@ -43,7 +48,28 @@ def needs_rebuild() -> bool:
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def build_host(force: bool = False) -> str:
+    if not force and os.path.exists(HOST_PATH) and os.path.getmtime(HOST_PATH) >= os.path.getmtime(HOST_SOURCE):
+        return HOST_PATH
+    import torch
+
+    os.makedirs(LIB_DIR, exist_ok=True)
+    base, tmp = os.path.dirname(torch.__file__), HOST_PATH + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I" + sysconfig.get_paths()["include"],
+           "-isystem", os.path.join(base, "include"),
+           "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           "-o", tmp, HOST_SOURCE, "-L" + os.path.join(base, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"g++ failed ({res.returncode}): {' '.join(cmd)}")
+    os.replace(tmp, HOST_PATH)
+    return HOST_PATH
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
+    build_host(force)
     if not force and not needs_rebuild():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import (KF_CACHE_BF16, KF_FLAG_CAUSAL, KF_FLAG_OUT_BF16, KF_FLAG_OUT_F16, KF_FLAG_Q_BF16,
-                   CallPlans, lib, on_device, strides_arg)
+                   CallPlans, host, host_plan, lib, on_device)
 
 __all__ = ["q4_cache", "kv_write_q4", "kv_read_q4", "flash_attn_paged_q4"]
 
@@ -85,19 +85,17 @@ def kv_write_q4(k, v, cache, slots, *, layout: str = "bhsd") -> None:
     strides (multiples of 8) with a contiguous head dimension.  slots: int32 ``[B, S]``; slot
     t is row ``t % block_size`` of block ``t // block_size``; one outside the cache (-1) is
     skipped.  Each head row is quantised by itself (scale and zero point per row)."""
-    key = (layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, cache.shape,
-           cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
-    plan = _write_plans.get(key) or _write_plans.put(key, _plan_io(cache, slots, k, v, layout))
-    index, dims, (_, strides), flags = plan
-    on_device(index, lib().kf_kv_write_q4, "kf_kv_write_q4", k.data_ptr(), v.data_ptr(), cache.data_ptr(),
-              slots.data_ptr(), *dims, strides, flags)
+    h = host()
+    key = (layout, h.form(k, v, cache, slots))
+    index, plan = _write_plans.get(key) or _write_plans.put(key, _plan_io(lib().kf_kv_write_q4, cache, slots, k, v, layout))
+    on_device(index, h.kv_io, "kf_kv_write_q4", plan, k, v, cache, slots)
 
 
 _write_plans, _read_plans, _attn_plans = CallPlans(), CallPlans(), CallPlans()
 
 
-def _plan_io(cache, slots, k, v, layout):
-    """Checks of a write or read and the arguments that follow from its tensors' form."""
+def _plan_io(fn, cache, slots, k, v, layout):
+    """Checks of a write or read (`fn`) and the arguments that follow from its tensors' form."""
     n_blocks, H_kv, bs, D = _cache_dims(cache)
     dev = cache.device
     (B, H, S, Dk), ks = _tokens(k, "k", layout, dev)
@@ -107,7 +105,7 @@ def _plan_io(cache, slots, k, v, layout):
     if (H, Dk) != (H_kv, D):
         raise ValueError(f"k and v must have the cache's {H_kv} heads of {D}")
     _check_slots(slots, B, S, dev)
-    return dev.index, (B, S, H, D, n_blocks, bs), strides_arg(*ks, *vs), _IO_FLAGS[k.dtype]
+    return dev.index, host_plan(fn, (*ks, *vs), (B, S, H, D, n_blocks, bs), _IO_FLAGS[k.dtype])
 
 
 def kv_read_q4(cache, slots, *, dtype=torch.float16, layout: str = "bhsd", out=None):
@@ -115,21 +113,17 @@ def kv_read_q4(cache, slots, *, dtype=torch.float16, layout: str = "bhsd", out=N
 
     ``[B, H_kv, S, D]`` ("bhsd", what :func:`flash_attn_fwd` takes) or ``[B, S, H_kv, D]``
     ("bshd").  A slot outside the cache reads zeros.  ``out``: (k, v) to write into."""
+    h = host()
     if out is None:
-        key = (layout, dtype, cache.shape, cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(),
-               slots.dtype, slots.device)
-        plan = _read_plans.get(key) or _read_plans.put(key, _plan_read(cache, slots, dtype, layout))
-        shape, device, (index, dims, (_, strides), flags) = plan
+        key = (layout, dtype, h.form(cache, slots))
+        shape, device, index, plan = _read_plans.get(key) or _read_plans.put(key, _plan_read(cache, slots, dtype, layout))
         k = torch.empty(shape, dtype=dtype, device=device)
         v = torch.empty_like(k)
     else:
         k, v = out
-        key = (layout, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, cache.shape,
-               cache.stride(), cache.dtype, cache.device, slots.shape, slots.stride(), slots.dtype, slots.device)
-        plan = _read_plans.get(key) or _read_plans.put(key, _plan_io(cache, slots, k, v, layout))
-        index, dims, (_, strides), flags = plan
-    on_device(index, lib().kf_kv_read_q4, "kf_kv_read_q4", cache.data_ptr(), slots.data_ptr(), k.data_ptr(),
-              v.data_ptr(), *dims, strides, flags)
+        key = (layout, h.form(cache, slots, k, v))
+        index, plan = _read_plans.get(key) or _read_plans.put(key, _plan_io(lib().kf_kv_read_q4, cache, slots, k, v, layout))
+    on_device(index, h.kv_io, "kf_kv_read_q4", plan, cache, slots, k, v)
     return k, v
 
 
@@ -144,8 +138,8 @@ def _plan_read(cache, slots, dtype, layout):
         shape, strides = (B, H_kv, S, D), (H_kv * S * D, S * D, D)
     else:
         shape, strides = (B, S, H_kv, D), (H_kv * S * D, D, H_kv * D)
-    return shape, cache.device, (cache.device.index, (B, S, H_kv, D, n_blocks, bs), strides_arg(*strides, *strides),
-                                 _IO_FLAGS[dtype])
+    return shape, cache.device, cache.device.index, host_plan(lib().kf_kv_read_q4, strides + strides,
+                                                              (B, S, H_kv, D, n_blocks, bs), _IO_FLAGS[dtype])
 
 
 def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=None, out=None, out_dtype=None,
@@ -164,21 +158,18 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
         out = torch.empty_like(q, dtype=out_dtype) if out_dtype is not None else torch.empty_like(q)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise ValueError("out and out_dtype disagree")
-    key = (causal, q.shape, q.stride(), q.dtype, q.device, cache.shape, cache.stride(), cache.dtype, cache.device,
-           block_table.shape, block_table.stride(), block_table.dtype, block_table.device, seq_lens.shape,
-           seq_lens.stride(), seq_lens.dtype, seq_lens.device, out.shape, out.stride(), out.dtype, out.device)
-    plan = _attn_plans.get(key) or _attn_plans.put(key, _plan_attn(q, cache, block_table, seq_lens, out, causal))
-    device, dims, flags, need = plan
+    h = host()
+    key = (bool(causal), h.form(q, cache, block_table, seq_lens, out))
+    device, index, need, plan = (_attn_plans.get(key) or
+                                 _attn_plans.put(key, _plan_attn(q, cache, block_table, seq_lens, out, causal)))
     if workspace is None:
         workspace = _workspace(device, need)
     Mi = Li = None
     if return_lse:
         Mi = torch.empty(q.shape[:3], dtype=torch.float32, device=device)
         Li = torch.empty_like(Mi)
-    on_device(device.index, lib().kf_attn_fwd_paged_q4, "kf_attn_fwd_paged_q4", q.data_ptr(), cache.data_ptr(),
-              block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), Mi.data_ptr() if return_lse else None,
-              Li.data_ptr() if return_lse else None, *dims, 0.0 if scale is None else scale, flags,
-              workspace.data_ptr(), workspace.numel())
+    on_device(index, h.attn_q4, "kf_attn_fwd_paged_q4", plan, q, cache, block_table, seq_lens, out, Mi, Li,
+              0.0 if scale is None else scale, workspace)
     return (out, Mi, Li) if return_lse else out
 
 
@@ -200,4 +191,5 @@ def _plan_attn(q, cache, block_table, seq_lens, out, causal):
     flags = (KF_FLAG_CAUSAL if causal else 0) | _OUT_FLAGS[out.dtype] | (KF_FLAG_Q_BF16 if q.dtype == torch.bfloat16 else 0)
     with torch.cuda.device(dev):
         need = lib().kf_attn_paged_q4_workspace_bytes(B, H_q, H_kv, S_q, D, bs, max_blocks)
-    return dev, (B, H_q, H_kv, S_q, D, n_blocks, bs, max_blocks), flags, max(need, 16)
+    return dev, dev.index, max(need, 16), host_plan(lib().kf_attn_fwd_paged_q4, (),
+                                                    (B, H_q, H_kv, S_q, D, n_blocks, bs, max_blocks), flags)

@@ -12,7 +12,7 @@ import ctypes
 
 import torch
 
-from ._lib import KF_PW_BF16, KF_ROPE_GPTJ, CallPlans, check, lib, on_device, strides_arg
+from ._lib import KF_PW_BF16, KF_ROPE_GPTJ, CallPlans, check, host, host_plan, lib, on_device
 
 __all__ = ["rms_norm", "fused_add_rms_norm", "rope_", "qk_norm_rope", "swiglu"]
 
@@ -147,24 +147,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
         out = (torch.empty_like(q, memory_format=torch.contiguous_format),
                torch.empty_like(k, memory_format=torch.contiguous_format) if k is not None else None)
     q_out, k_out = out
-    key = (layout, interleaved, rot_dim, q.shape, q.stride(), q.dtype, q.device, q_out.shape, q_out.stride(), q_out.dtype,
-           q_out.device, _form(k), _form(k_out), _form(q_weight), _form(k_weight), _form(positions), _form(inv_freq))
-    plan = _qk_plans.get(key) or _qk_plans.put(key, _plan_qk_norm_rope(
+    hs = host()
+    key = (layout, bool(interleaved), rot_dim, hs.form(q, k, q_weight, k_weight, q_out, k_out, positions, inv_freq))
+    index, plan = _qk_plans.get(key) or _qk_plans.put(key, _plan_qk_norm_rope(
         q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq, layout, interleaved, rot_dim))
-    index, (B, S, H_q, H_kv, D, rot), (_, strides), flags = plan
-    on_device(index, lib().kf_qk_norm_rope, "kf_qk_norm_rope", q.data_ptr(), k.data_ptr() if k is not None else None,
-              q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
-              q_out.data_ptr(), k_out.data_ptr() if k_out is not None else None,
-              positions.data_ptr() if positions is not None else None, inv_freq.data_ptr() if inv_freq is not None else None,
-              B, S, H_q, H_kv, D, rot, theta, rot_scale, eps, strides, flags)
+    on_device(index, hs.qk_norm_rope, "kf_qk_norm_rope", plan, q, k, q_weight, k_weight, q_out, k_out, positions, inv_freq,
+              theta, rot_scale, eps)
     return q_out, k_out
 
 
 _qk_plans = CallPlans()
-
-
-def _form(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 def _plan_qk_norm_rope(q, q_out, k, k_out, q_weight, k_weight, positions, inv_freq, layout, interleaved, rot_dim):
@@ -206,8 +198,8 @@ def _plan_qk_norm_rope(q, q_out, k, k_out, q_weight, k_weight, positions, inv_fr
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.numel() != rot // 2
                                  or not inv_freq.is_contiguous() or inv_freq.device != dev):
         raise ValueError("inv_freq must be a contiguous float32 [rot_dim/2] tensor on q's device")
-    return (dev.index, (B, S, heads[0], heads[1], D, rot), strides_arg(*strides[0], *strides[1]),
-            flag | (KF_ROPE_GPTJ if interleaved else 0))
+    return dev.index, host_plan(lib().kf_qk_norm_rope, strides[0] + strides[1], (B, S, heads[0], heads[1], D, rot),
+                                flag | (KF_ROPE_GPTJ if interleaved else 0))
 
 
 def swiglu(gate_up: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
