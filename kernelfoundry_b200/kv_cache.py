@@ -153,7 +153,8 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
     ``H_q / H_kv * S_q <= 64``.  O has ``out_dtype`` (or ``out``'s; default q's dtype);
     with ``return_lse`` also (Mi, Li), the row max of the scaled scores and sum of exp(s - Mi).
     Each stream has its workspace; ``workspace`` (zero-filled uint8,
-    ``kf_attn_paged_q4_workspace_bytes``) replaces it, e.g. for a captured graph."""
+    ``kf_attn_paged_q4_workspace_bytes``) replaces it: a captured graph that may run beside other
+    calls, or other graphs captured on its stream, needs one of its own."""
     if out is None:
         out = torch.empty_like(q, dtype=out_dtype) if out_dtype is not None else torch.empty_like(q)
     elif out_dtype is not None and out.dtype != out_dtype:
