@@ -67,9 +67,9 @@ int kf_kv_read_q4(const void* cache, const int* slots, void* k, void* v, int B, 
  * KF_FLAG_OUT_F16 / KF_FLAG_OUT_BF16 (default fp32 O).  A query row that sees no key gets
  * O = 0 (Mi = -inf, Li = 0).  Mi / Li (optional) as kf_attn_fwd_lse.  scale == 0: 1/sqrt(D).
  * Table entries past a sequence's last block are not read; an entry outside
- * [0, n_blocks) reads zeros.  Probabilities, times the values' scales, enter the second
- * product as fp16 for a bf16 O (2^-11 a key, relative) and as two fp16 for fp16 and fp32 (2^-22);
- * everything else is exact or fp32.  max_blocks * block_size < 2^31 - 64.
+ * [0, n_blocks) reads zeros.  Probabilities times the values' scales enter the second
+ * product as fp16 for a bf16 O (2^-11 a key, relative) and as two fp16 for fp16 and fp32 (2^-22),
+ * in both cases to no finer than 2^-23 of the row's largest; everything else is exact or fp32.  max_blocks * block_size < 2^31 - 64.
  * workspace: required, kf_attn_paged_q4_workspace_bytes(), handled as kf_attn_fwd's
  * (zero-filled once, left ready by every call, not shared by overlapping calls);
  * KF_ERR_WORKSPACE if it is too small. */

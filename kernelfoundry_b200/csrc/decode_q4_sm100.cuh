@@ -21,13 +21,16 @@
 // value's own size, where sum(p t n) - sum(p t z) would cancel.
 // Queries are scaled by a power of two per row to a maximum in [2^13, 2^14), which holds fp16
 // rows exactly, and bf16 ones but for elements below 2^-28 of the row's largest.
-// p t enters the second product as fp16, scaled by a power of two such that the largest t seen
-// stays below 2^7 (t spans any range; small ones lose bits only against the largest).  For a
-// bf16 output this rounding, 2^-11 relative per key, is the only one below fp32 in the sum; for
-// fp16 and fp32 outputs (SPLIT) what it leaves goes in as a second fp16 operand, which leaves 2^-22.
-// The running maximum is lazy: p = 2^(x - m) with an m that is raised only when a score passes
+// p t enters the second product as fp16, times a power of two (norm) of its query row: the one that
+// keeps the largest t seen below 2^7, or a larger one if the row's largest p t would then be below
+// 2^-2 (a value far beyond the others with next to no probability, or hidden from the row, must not
+// push the others out of fp16).  For a bf16 output this rounding is the only one below fp32 in the
+// sum, 2^-11 relative per key (or 2^-23 of the row's largest p t); for fp16 and fp32 outputs (SPLIT)
+// what it leaves goes in as a second fp16 operand, which leaves 2^-22 (or the same 2^-23).
+// The running maximum is lazy: p = 2^(x - m) with an integer m that is raised only when a score passes
 // m + 8 (p <= 2^8 then, which fp16 and fp32 hold as well as p <= 1), so a tile needs one vote
-// instead of a maximum across the warp.  The true maximum is kept per thread and put in at the end.
+// instead of a maximum across the warp, and the same vote finds a t beyond what the norms allow.
+// The true maximum is kept per thread and put in at the end.
 //
 // Work split.  Every (sequence, cache head, group of 8 NT query rows) is a unit of 32-key
 // tiles; all units' tiles in a row (and kQ4UnitTiles more for each unit) are cut evenly over the CTAs (one per SM) and each CTA's
@@ -146,9 +149,12 @@ struct Q4Warp {                    // a warp's running state of one unit; pairs:
     float2 mt[NT];                 // this thread's largest score
     uint32_t q[NT][Q4AttnCfg<D, NT>::KW][4];
     float2 qs[NT], cq[NT];         // -sum(q) * 2^-22, and a column's factor of the scores
-    float tmx;                     // this thread's largest value scale
-    float tlim, tnorm, tinv;       // value scales up to tlim times tnorm stay below 2^7; tinv = 1 / tnorm
+    float2 norm[NT];               // a column's factor of p t, a power of two
+    float tlim;                    // value scales up to tlim times this thread's norms stay within 2^7
 };
+
+__device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }   // 2^(e - 127)
+constexpr int kQ4NormMin = 6, kQ4NormMax = 233;                  // biased exponents of norm: 2^-121, 2^106
 
 __device__ __forceinline__ float2 fmax2(float2 a, float2 b) { return make_float2(fmaxf(a.x, b.x), fmaxf(a.y, b.y)); }
 
@@ -199,8 +205,7 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
                                          const Q4Cursor& c, int lane) {
     using C = Q4AttnCfg<D, NT>;
     const int t = lane & 3;
-    s.tmx = s.tlim = 0.f;
-    s.tnorm = s.tinv = 1.0f;
+    s.tlim = pow2_biased(261 - kQ4NormMax);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         float x[C::KW][8], mx = 0.f, sum = 0.f;
@@ -235,6 +240,7 @@ __device__ __forceinline__ void q4_begin(const Q4AttnParams& p, Q4Warp<D, NT>& s
         s.m[n] = make_float2(kQ4NoMax, kQ4NoMax);
         s.mt[n] = make_float2(-INFINITY, -INFINITY);
         s.l[n] = make_float2(0.f, 0.f);
+        s.norm[n] = make_float2(pow2_biased(kQ4NormMax), pow2_biased(kQ4NormMax));
 #pragma unroll
         for (int i = 0; i < C::MT; ++i)
 #pragma unroll
@@ -324,10 +330,9 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
             }
         }
     }
-    // Does a score pass m + 8, or a value scale the range of p t?  Rarely.
-    s.tmx = fmax3f(s.tmx, tv[0][0], tv[0][1]);                               // (a spoiled row's NaN is ignored)
-    s.tmx = fmax3f(s.tmx, tv[1][0], tv[1][1]);
-    bool up = s.tmx > s.tlim;
+    // Does a score pass m + 8, or a value scale what the norms are good for?  Rarely.
+    const float tm = fmax3f(fmax3f(tv[0][0], tv[0][1], tv[1][0]), tv[1][1], 0.f);   // (a spoiled row's NaN is ignored)
+    bool up = tm > s.tlim;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         s.mt[n].x = fmax3f(fmax3f(s.mt[n].x, x[0][n][0].x, x[0][n][1].x), x[1][n][0].x, x[1][n][1].x);
@@ -335,40 +340,50 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
         up = up || s.mt[n].x > s.m[n].x + 8.0f || s.mt[n].y > s.m[n].y + 8.0f;
     }
     if (__any_sync(0xffffffffu, up)) {
-        const float tt = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s.tmx)));
-        float r = 1.0f;
-        if (tt > s.tlim) {
-            int e = static_cast<int>(__float_as_uint(tt) >> 23);             // 27 or more: scales are 0 or >= 2^-100
-            e = e < 7 ? 7 : e;                                               // (but the bytes are the caller's)
-            s.tlim = __uint_as_float(static_cast<uint32_t>(e < 254 ? e + 1 : 254) << 23);
-            s.tnorm = __uint_as_float(static_cast<uint32_t>(260 - e) << 23);  // 2^6 / 2^(e - 127)
-            r = s.tnorm * s.tinv;
-            s.tinv = __uint_as_float(static_cast<uint32_t>(e - 6) << 23);
-        }
+        const int et = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(tm)) >> 23);
+        int top = 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float v[2] = {s.mt[n].x, s.mt[n].y}, a[2];
+            float v[2] = {s.mt[n].x, s.mt[n].y}, a[2], r[2], nm[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const float m = k ? s.m[n].y : s.m[n].x;
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 4));
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 8));
                 v[k] = fmaxf(v[k], __shfl_xor_sync(0xffffffffu, v[k], 16));
-                v[k] = fmaxf(v[k], m);                                       // (no key seen by this column yet: kQ4NoMax)
-                a[k] = ex2_approx(m - v[k]);
+                v[k] = fmaxf(ceilf(v[k]), m);                                // (no key seen by this column yet: kQ4NoMax)
+                float pt = 0.f;                                              // the tile's largest p t that the column sees
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        pt = fmaxf(pt, ex2_approx((k ? x[j][n][h].y : x[j][n][h].x) - v[k]) * tv[j][h]);
+                pt = fmaxf(pt, __shfl_xor_sync(0xffffffffu, pt, 4));
+                pt = fmaxf(pt, __shfl_xor_sync(0xffffffffu, pt, 8));
+                pt = fmaxf(pt, __shfl_xor_sync(0xffffffffu, pt, 16));
+                const int d = static_cast<int>(fminf(v[k] - m, 512.0f));     // m moves by whole powers of two
+                const int was = static_cast<int>(__float_as_uint(k ? s.norm[n].y : s.norm[n].x) >> 23);
+                int e = 260 - et;                                            // t norm < 2^7 ...
+                e = max(e, pt > 0.f ? 252 - static_cast<int>(__float_as_uint(pt) >> 23) : 0);   // ... but p t norm >= 2^-2
+                e = max(min(min(e, was + d), kQ4NormMax), kQ4NormMin);       // O is never scaled up
+                const int er = 127 - d + e - was;
+                top = max(top, e);
+                nm[k] = pow2_biased(e);
+                a[k] = d < 127 ? pow2_biased(127 - d) : 0.f;
+                r[k] = er > 0 ? pow2_biased(er) : 0.f;
             }
             s.m[n] = make_float2(v[0], v[1]);
+            s.norm[n] = make_float2(nm[0], nm[1]);
             s.l[n] = make_float2(s.l[n].x * a[0], s.l[n].y * a[1]);
-            a[0] *= r;
-            a[1] *= r;
 #pragma unroll
             for (int i = 0; i < C::MT; ++i) {
-                s.o[n][i][0] *= a[0];
-                s.o[n][i][1] *= a[1];
-                s.o[n][i][2] *= a[0];
-                s.o[n][i][3] *= a[1];
+                s.o[n][i][0] *= r[0];
+                s.o[n][i][1] *= r[1];
+                s.o[n][i][2] *= r[0];
+                s.o[n][i][3] *= r[1];
             }
         }
+        s.tlim = pow2_biased(261 - top);                                     // 2^7 / the larger norm
     }
     // O^T += V^T P^T
 #pragma unroll
@@ -378,13 +393,12 @@ __device__ __forceinline__ void q4_tile(const Q4AttnParams& p, Q4Warp<D, NT>& s,
         uint32_t pb[NT][2], pl[NT][2];                                       // p t, and (SPLIT) what its rounding left
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float tn = tv[j][h] * s.tnorm;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float2 d = fadd2(x[j][n][h], make_float2(-s.m[n].x, -s.m[n].y));
                 const float2 pr = make_float2(ex2_approx(d.x), ex2_approx(d.y));
                 s.l[n] = fadd2(s.l[n], pr);
-                float2 pt = fmul2(pr, make_float2(tn, tn));
+                float2 pt = fmul2(fmul2(pr, make_float2(tv[j][h], tv[j][h])), s.norm[n]);
                 if (MASKED) {                                                // 0 * a spoiled row's NaN
                     const int key = key0 + 16 * j + 8 * h + g;
                     if (key >= lim[n][0]) pt.x = 0.f;
@@ -486,7 +500,8 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
         const float2 a = make_float2(m.x == -INFINITY ? 1.0f : ex2_approx(s.m[n].x - m.x),
                                      m.y == -INFINITY ? 1.0f : ex2_approx(s.m[n].y - m.y));
         l = fmul2(l, a);
-        float2 f = fmul2(a, make_float2(s.tinv, s.tinv));
+        float2 f = fmul2(a, make_float2(pow2_biased(254 - static_cast<int>(__float_as_uint(s.norm[n].x) >> 23)),
+                                        pow2_biased(254 - static_cast<int>(__float_as_uint(s.norm[n].y) >> 23))));
         if (whole) f = fmul2(f, make_float2(l.x == 0.f ? 0.f : 1.0f / l.x, l.y == 0.f ? 0.f : 1.0f / l.y));
         const int col = 8 * n + 2 * t;
 #pragma unroll

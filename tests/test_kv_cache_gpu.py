@@ -326,6 +326,82 @@ def test_scale_growing_maximum_and_outlier_scales(cuda):
         _check(_attn(cuda, q, "bf16", cache, table, [n], scale=scale, out_dtype=_tdt("f32")), O, A, "f32", f"scale {scale}")
 
 
+def _with_rows(cache, table, bs, b, rows):
+    """``cache`` with rows {key: (k or None, v or None)} of sequence b rewritten for every head (bf16 values, [D])."""
+    H, D = cache.shape[1], cache.shape[-1] // 16 - 8
+    for j, (k, v) in rows.items():
+        t = int(table[b, j // bs] * bs + j % bs)
+        old = [x[0, :, 0] for x in qo.read(cache, np.array([[t]]))]
+        k, v = (po.round_to(np.broadcast_to(o if x is None else x, (H, D)), "bf16") for x, o in zip((k, v), old))
+        cache = qo.write(cache, np.array([[t]], np.int32), k[None, :, None].astype(np.float32), v[None, :, None].astype(np.float32))
+    return cache
+
+
+def _check_rows(got, O, A, out_dt, what):
+    """Outputs where one value row is far larger than the others.  p t (t: a value's scale) is rounded per key as
+    elsewhere (within 2^-10 A), and by 2^-23 of the row's largest p t, as fp16 has a last bit.  The key with that
+    largest one adds at least 7 times it to A in some dim, and a rounding moves an output by at most 15 times
+    itself: 2^-21.9 max_d A a key, as many as 2^7 times that for 3000 independent ones: below 2^-13 max_d A."""
+    got = _host(got)
+    half_ulp = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 2.0 ** -24}[out_dt]
+    tol = 2.0 ** -10 * A + 2.0 ** -13 * A.max(-1, keepdims=True) + half_ulp * np.abs(O) + (2.0 ** -25 if out_dt == "f16" else 0.0)
+    bad = ~(np.abs(got - O) <= tol)
+    assert not bad.any(), f"{what}: {bad.sum()} outside, worst {np.nanmax(np.abs(got - O) / np.maximum(tol, 1e-30)):.2f}x"
+
+
+@pytest.mark.parametrize("out_dt", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("D,H_q,S_q", [(64, 4, 2), (64, 8, 2), (128, 4, 2), (128, 4, 4), (256, 2, 3)])
+def test_a_huge_value_hidden_from_a_row_leaves_it_alone(cuda, D, H_q, S_q, out_dt):
+    """The last draft's value is 1e20 (or 1e7): earlier drafts, which may not see it, are what they are without it."""
+    rng = np.random.default_rng(40 + D + S_q)
+    for n, big in ((40, 1e20), (40, 1e7), (3000, 1e20)):
+        cache, table = _filled(rng, 1, 1, D, 16, [n])
+        cache = _with_rows(cache, table, 16, 0, {n - 1: (None, np.full(D, big) * rng.uniform(0.5, 1, D))})
+        q = po.round_to(rng.standard_normal((1, H_q, S_q, D)), "bf16")
+        O, _, _, A = qo.attention(q, cache, table, [n], causal=True)
+        got = _attn(cuda, q, "bf16", cache, table, [n], causal=True, out_dtype=_tdt(out_dt))
+        if out_dt == "f16":                              # rows that see it are beyond fp16
+            assert np.isinf(_host(got)[:, :, -1]).any() or big == 1e7
+            got, O, A = got[:, :, :-1], O[:, :, :-1], A[:, :, :-1]
+        _check_rows(got, O, A, out_dt, f"n {n}, value {big}")
+
+
+@pytest.mark.parametrize("out_dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [30, 2000])
+@pytest.mark.parametrize("at", ["first", "last"])
+def test_a_huge_value_with_next_to_no_probability(cuda, n, at, out_dt):
+    """One key scores 60 below the maximum and its value is 1e20: it adds about 1e-6, the others stay what they are."""
+    D = 128
+    rng = np.random.default_rng(50 + n)
+    cache, table = _filled(rng, 1, 1, D, 16, [n])
+    u = np.sign(rng.standard_normal(D))                  # scores: key . q / sqrt(D), q = u
+    j = 0 if at == "first" else n - 1
+    rows = {j: (-45 / np.sqrt(D) * u, np.full(D, 1e20) * rng.uniform(0.5, 1, D)), n // 2: (15 / np.sqrt(D) * u, None)}
+    cache = _with_rows(cache, table, 16, 0, rows)
+    q = po.round_to(np.stack([u, 0.5 * u, 0.25 * u, -0.1 * u])[None, :, None], "bf16")
+    O, _, _, A = qo.attention(q, cache, table, [n])
+    assert A[0, 0].max() < 100 < A[0, 3].max()           # negligible in the first row, everything in the last
+    _check_rows(_attn(cuda, q, "bf16", cache, table, [n], out_dtype=_tdt(out_dt)), O, A, out_dt, at)
+
+
+@pytest.mark.parametrize("out_dt", ["bf16", "f32"])
+@pytest.mark.parametrize("tiny", [1.0, 1e-6, 1e-12])
+@pytest.mark.parametrize("B,n", [(1500, 256), (1, 3000)])
+def test_early_huge_values_outweighed_by_later_scores(cuda, B, n, tiny, out_dt):
+    """Values of 1e15 lead while the scores are low; later keys outweigh the first of them by 2^115, with ordinary and with
+    tiny values.  1500 sequences on the same pages give a warp whole units of 8 tiles, one sequence is split over all warps."""
+    D, H = 128, 2
+    rng = np.random.default_rng(60)
+    cache, table = _filled(rng, 1, H, D, 16, [n])
+    u = np.sign(rng.standard_normal(D))
+    step = np.linspace(-40, 40, n)
+    rows = {j: (step[j] / np.sqrt(D) * u, rng.standard_normal(D) * (1e15 if j < n // 4 else tiny)) for j in range(0, n, max(1, n // 256))}
+    cache = _with_rows(cache, table, 16, 0, rows)
+    q = po.round_to(np.stack([u, -u, 0.3 * u, 0 * u])[None, :, None], "bf16")
+    O, _, _, A = qo.attention(q, cache, table, [n])
+    got = _attn(cuda, np.repeat(q, B, 0), "bf16", cache, np.repeat(table, B, 0), [n] * B, out_dtype=_tdt(out_dt))
+    _check_rows(got, O, A, out_dt, "")
+
 def test_query_magnitudes(cuda):
     """bf16 rows far apart in size (beyond fp16's range) in one call; a zero row attends uniformly."""
     rng = np.random.default_rng(12)
