@@ -45,12 +45,21 @@ class Q4AttentionBlock:
         self.cache = q4_cache(batch * per, H_kv, block_size, D, self.device)
         self.table = torch.randperm(batch * per, generator=g, device=self.device).to(torch.int32).view(batch, per)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self.capacity = per * block_size                   # tokens of a sequence that the table has room for
+        self._most = 0                                     # what the longest sequence has, or more: the lengths are on the device
 
     def slots(self, positions, valid=None):
-        """Cache slots of ``positions`` [B, S] (int64); -1 where not valid."""
-        blocks = self.table.gather(1, positions // self.block_size).long()
-        s = blocks * self.block_size + positions % self.block_size
-        return (s if valid is None else s.masked_fill(~valid, -1)).to(torch.int32)
+        """Cache slots of ``positions`` [B, S] (int64); -1 where not valid and past the table (padding may be there)."""
+        page = positions // self.block_size
+        outside = page >= self.table.shape[1]
+        if valid is not None:
+            outside = outside | ~valid
+        blocks = self.table.gather(1, page.clamp(max=self.table.shape[1] - 1)).long()
+        return (blocks * self.block_size + positions % self.block_size).masked_fill(outside, -1).to(torch.int32)
+
+    def _check_room(self, n):
+        if n > self.capacity:
+            raise ValueError(f"a sequence would have {n} tokens, the block table has room for {self.capacity}")
 
     def _project(self, x, positions):
         """Rotated queries and keys, and values, all [B, H, S, D]."""
@@ -72,8 +81,12 @@ class Q4AttentionBlock:
     def prefill(self, x, lens=None, past: int = 0):
         """A chunk ``x`` [B, S, hidden] at positions past ..; ``lens`` [B]: tokens of each (the rest is padding).
 
-        Every sequence has ``past`` tokens in the cache already; they are read back and attended."""
+        Every sequence has ``past`` tokens in the cache already; they are read back and attended.  Padding may go
+        past the table, a token may not (ValueError)."""
         B, S, _ = x.shape
+        if past + S > self.capacity:
+            self._check_room(past + (S if lens is None else int(lens.max())))
+        self._most = past + S
         positions = past + torch.arange(S, device=x.device).expand(B, S)
         lens = torch.full((B,), S, dtype=torch.int32, device=x.device) if lens is None else lens
         q, k, v = self._project(x, positions)
@@ -88,8 +101,18 @@ class Q4AttentionBlock:
         return self._output(x, o)
 
     def step(self, x):
-        """``x`` [B, S, hidden]: the next S tokens of every sequence (S > 1: drafts, causal among themselves)."""
+        """``x`` [B, S, hidden]: the next S tokens of every sequence (S > 1: drafts, causal among themselves).
+
+        ValueError if they do not fit the table.  Replays of a captured step are the caller's to count: nothing on
+        the host sees them, and a token past the table is not kept."""
         B, S, _ = x.shape
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            self._most = self.capacity                     # from here on the lengths are looked at
+        else:
+            if self._most + S > self.capacity:
+                self._most = int(self.lens.max())
+                self._check_room(self._most + S)
+            self._most += S
         positions = self.lens.long()[:, None] + torch.arange(S, device=x.device)
         q, k, v = self._project(x, positions)
         kv_write_q4(k, v, self.cache, self.slots(positions))
