@@ -47,6 +47,7 @@ class Q4AttentionBlock:
         self.lens = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.capacity = per * block_size                   # tokens of a sequence that the table has room for
         self._most = 0                                     # what the longest sequence has, or more: the lengths are on the device
+        self._captured = False                             # a graph's replays may have moved them since
 
     def slots(self, positions, valid=None):
         """Cache slots of ``positions`` [B, S] (int64); -1 where not valid and past the table (padding may be there)."""
@@ -107,9 +108,9 @@ class Q4AttentionBlock:
         the host sees them, and a token past the table is not kept."""
         B, S, _ = x.shape
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            self._most = self.capacity                     # from here on the lengths are looked at
+            self._captured = True
         else:
-            if self._most + S > self.capacity:
+            if self._captured or self._most + S > self.capacity:
                 self._most = int(self.lens.max())
                 self._check_room(self._most + S)
             self._most += S

@@ -45,3 +45,12 @@ def test_step_refuses_what_does_not_fit():
         with pytest.raises(ValueError, match="room for 112"):
             block.step(torch.zeros(3, S, 64).half())
         assert block.lens.tolist() == lens
+
+
+def test_steps_after_a_capture_look_at_the_lengths():
+    """Replays move the lengths unseen: the host's own count says nothing any more."""
+    block = _block()
+    block._captured = True
+    block.lens.copy_(torch.tensor([112, 0, 0]))
+    with pytest.raises(ValueError, match="room for 112"):
+        block.step(torch.zeros(3, 1, 64).half())
