@@ -78,6 +78,11 @@ def _workspace(device, nbytes):
     return ws
 
 
+def _check_workspace(workspace, device):
+    if workspace.device != device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on {device}")
+
+
 def kv_write_q4(k, v, cache, slots, *, layout: str = "bhsd") -> None:
     """Quantise ``k`` and ``v`` to 4 bits into ``cache``: token (b, s) goes to slot ``slots[b, s]``.
 
@@ -165,6 +170,8 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
                                  _attn_plans.put(key, _plan_attn(q, cache, block_table, seq_lens, out, causal)))
     if workspace is None:
         workspace = _workspace(device, need)
+    else:
+        _check_workspace(workspace, device)
     Mi = Li = None
     if return_lse:
         Mi = torch.empty(q.shape[:3], dtype=torch.float32, device=device)

@@ -105,3 +105,18 @@ def test_oracle_attention_equals_a_direct_softmax():
         p = np.exp(s - s.max())
         np.testing.assert_allclose(O[0, h, i], p @ vq[:18 + i] / p.sum(), rtol=1e-12)
         assert np.isclose(Mi[0, h, i], s.max()) and np.isclose(Li[0, h, i], p.sum())
+
+
+def test_workspace_form(kf_lib):
+    """A workspace elsewhere, of another type or with gaps never reaches the kernel."""
+    import pytest
+    import torch
+
+    from kernelfoundry_b200.kv_cache import _check_workspace
+
+    here, there = torch.device("cpu"), torch.device("meta")
+    _check_workspace(torch.zeros(64, dtype=torch.uint8), here)
+    for ws, dev in ((torch.zeros(64, dtype=torch.uint8), there), (torch.zeros(64, dtype=torch.float32), here),
+                    (torch.zeros(128, dtype=torch.uint8)[::2], here)):
+        with pytest.raises(ValueError, match="workspace"):
+            _check_workspace(ws, dev)

@@ -599,3 +599,25 @@ def test_refusals(cuda):
         flash_attn_paged_q4(q, c, t, n, scale=float("nan"))
     e = torch.zeros(0, 4, 1, 128, device=cuda, dtype=torch.float16)
     assert flash_attn_paged_q4(e, c, t[:0], n[:0]).shape == e.shape
+
+
+def test_refused_workspaces(cuda):
+    """Refused on the host, also once a call of the same form has gone through; a good one still does."""
+    import torch
+
+    from kernelfoundry_b200 import KFError, flash_attn_paged_q4, q4_cache
+    from kernelfoundry_b200.attention import new_workspace
+
+    q = torch.zeros(1, 4, 1, 128, device=cuda, dtype=torch.float16)
+    args = (q, q4_cache(4, 2, 16, 128, cuda), torch.zeros(1, 4, device=cuda, dtype=torch.int32),
+            torch.full((1,), 5, device=cuda, dtype=torch.int32))
+    n = 1 << 22
+    good = new_workspace(n, cuda)
+    want = flash_attn_paged_q4(*args, workspace=good)
+    for bad in (torch.zeros(n, dtype=torch.uint8), torch.zeros(n, dtype=torch.uint8).pin_memory(),
+                torch.zeros(n, device=cuda), torch.zeros(2 * n, dtype=torch.uint8, device=cuda)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            flash_attn_paged_q4(*args, workspace=bad)
+    with pytest.raises(KFError):
+        flash_attn_paged_q4(*args, workspace=good[:1024])
+    assert torch.equal(flash_attn_paged_q4(*args, workspace=good), want)
