@@ -140,7 +140,7 @@ struct Q4Cursor {
     int nt, len;                   // the sequence's tiles and keys
 };
 
-constexpr float kQ4NoMax = -1e30f;
+constexpr float kQ4NoMax = -3.402823466e38f;                    // below every finite score
 
 template <int D, int NT>
 struct Q4Warp {                    // a warp's running state of one unit; pairs: columns 2t, 2t + 1

@@ -402,6 +402,23 @@ def test_early_huge_values_outweighed_by_later_scores(cuda, B, n, tiny, out_dt):
     got = _attn(cuda, np.repeat(q, B, 0), "bf16", cache, np.repeat(table, B, 0), [n] * B, out_dtype=_tdt(out_dt))
     _check_rows(got, O, A, out_dt, "")
 
+def test_scores_of_any_size(cuda):
+    """Scores near +-1e36 (bf16 queries and keys): equal keys weigh alike whatever the sign, a lower one nothing."""
+    D = 64
+    rng = np.random.default_rng(30)
+    u = np.sign(rng.standard_normal(D))
+    for n in (1, 20, 70):
+        cache, table = _filled(rng, 1, 1, D, 16, [n])
+        cache = _with_rows(cache, table, 16, 0, {j: (2.0 ** 55 * u * (0.5 if j == 13 else 1.0), None) for j in range(n)})
+        q = po.round_to(np.stack([-u, u, 0.25 * u, -2.0 ** -100 * u])[None, :, None] * 2.0 ** 60, "bf16")
+        O, Mi, Li, A = qo.attention(q, cache, table, [n])
+        assert Mi.min() < -1e34 and Mi.max() > 1e34
+        got, mi, li = _attn(cuda, q, "bf16", cache, table, [n], out_dtype=_tdt("f32"), return_lse=True)
+        _check(got, O, A, "f32", f"n {n}")
+        assert (np.abs(_host(mi) - Mi) <= 2.0 ** -18 * np.maximum(np.abs(Mi), 1)).all()
+        assert (np.abs(_host(li) - Li) <= 2.0 ** -12 * Li).all()
+
+
 def test_query_magnitudes(cuda):
     """bf16 rows far apart in size (beyond fp16's range) in one call; a zero row attends uniformly."""
     rng = np.random.default_rng(12)
