@@ -12,6 +12,7 @@
 
 #include <cstring>
 #include <exception>
+#include <limits>
 
 namespace {
 
@@ -144,7 +145,10 @@ PyObject* attn_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         void *x[7], *ws = ptr(a[9]), *s = stream(a[10]);
         for (int i = 0; i < 7; ++i) x[i] = ptr(a[1 + i]);
         const size_t ws_bytes = a[9] == Py_None ? 0 : tensor(a[9]).nbytes();
-        const float scale = number(a[8]);
+        // None is the C function's 0, the default; a number that is 0 in fp32 becomes its smallest one, with which every
+        // score is as good as 0.
+        float scale = 0.0f;
+        if (a[8] != Py_None && (scale = number(a[8])) == 0.0f) scale = std::numeric_limits<float>::denorm_min();
         return status([&] {
             return reinterpret_cast<AttnFn>(p.fn)(x[0], x[1], static_cast<int*>(x[2]), static_cast<int*>(x[3]), x[4],
                                                   static_cast<float*>(x[5]), static_cast<float*>(x[6]), p.dims[0], p.dims[1],

@@ -154,7 +154,7 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
     block_table int32 ``[B, max_blocks]``: pool block of each logical block; seq_lens int32
     ``[B]``: keys per sequence (0 gives O = 0).  ``causal``: query i sees keys
     ``j <= seq_len - S_q + i`` (drafted tokens whose keys are already in the cache); a row
-    that sees no key is 0.  ``scale`` defaults to 1/sqrt(D).  Decode shapes:
+    that sees no key is 0.  ``scale`` defaults to 1/sqrt(D); 0 weighs all keys alike.  Decode shapes:
     ``H_q / H_kv * S_q <= 64``.  O has ``out_dtype`` (or ``out``'s; default q's dtype);
     with ``return_lse`` also (Mi, Li), the row max of the scaled scores and sum of exp(s - Mi).
     Each stream has its workspace; ``workspace`` (zero-filled uint8,
@@ -177,7 +177,7 @@ def flash_attn_paged_q4(q, cache, block_table, seq_lens, *, causal=False, scale=
         Mi = torch.empty(q.shape[:3], dtype=torch.float32, device=device)
         Li = torch.empty_like(Mi)
     on_device(index, h.attn_q4, "kf_attn_fwd_paged_q4", plan, q, cache, block_table, seq_lens, out, Mi, Li,
-              0.0 if scale is None else scale, workspace)
+              scale, workspace)
     return (out, Mi, Li) if return_lse else out
 
 

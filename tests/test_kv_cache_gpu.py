@@ -419,6 +419,18 @@ def test_scores_of_any_size(cuda):
         assert (np.abs(_host(li) - Li) <= 2.0 ** -12 * Li).all()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-60, 1e-30])
+def test_a_scale_of_zero_is_not_the_default(cuda, scale):
+    """scale=0 weighs all keys alike, and so does a scale too small for fp32; None is 1/sqrt(D)."""
+    rng = np.random.default_rng(31)
+    cache, table = _filled(rng, 2, 2, 128, 16, [75, 3])
+    q = po.round_to(3 * rng.standard_normal((2, 8, 1, 128)), "f16")
+    O, _, Li, A = qo.attention(q, cache, table, [75, 3], scale=scale)
+    got, mi, li = _attn(cuda, q, "f16", cache, table, [75, 3], scale=scale, return_lse=True)
+    _check(got, O, A, "f16")
+    assert np.abs(_host(mi)).max() < 1e-25 and (np.abs(_host(li) - Li) <= 2.0 ** -12 * Li).all()
+
+
 def test_query_magnitudes(cuda):
     """bf16 rows far apart in size (beyond fp16's range) in one call; a zero row attends uniformly."""
     rng = np.random.default_rng(12)
