@@ -18,6 +18,7 @@ import argparse
 
 import torch
 
+from ._lib import lib
 from .attention import flash_attn_fwd
 from .kv_cache import flash_attn_paged_q4, kv_read_q4, kv_write_q4, q4_cache
 from .pointwise import qk_norm_rope, rms_norm
@@ -48,6 +49,11 @@ class Q4AttentionBlock:
         self.capacity = per * block_size                   # tokens of a sequence that the table has room for
         self._most = 0                                     # what the longest sequence has, or more: the lengths are on the device
         self._captured = False                             # a graph's replays may have moved them since
+        # The attention's workspace, one for eager and captured steps alike (they share the cache, so they never overlap).
+        # Without it a call captured on a stream of the graph's own records a zero-fill of a new one.
+        most = max(1, 64 // max(1, H_q // H_kv))           # tokens of a step, at most
+        need = max(lib().kf_attn_paged_q4_workspace_bytes(batch, H_q, H_kv, s, D, block_size, per) for s in (1, most))
+        self._workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
 
     def slots(self, positions, valid=None):
         """Cache slots of ``positions`` [B, S] (int64); -1 where not valid and past the table (padding may be there)."""
@@ -118,7 +124,7 @@ class Q4AttentionBlock:
         q, k, v = self._project(x, positions)
         kv_write_q4(k, v, self.cache, self.slots(positions))
         self.lens += S
-        o = flash_attn_paged_q4(q, self.cache, self.table, self.lens, causal=S > 1)
+        o = flash_attn_paged_q4(q, self.cache, self.table, self.lens, causal=S > 1, workspace=self._workspace)
         return self._output(x, o)
 
 
@@ -147,7 +153,7 @@ def main(argv=None):
           "of the attention's contribution")
 
     static = token.clone()
-    block.step(static)                                     # warm-up: plans and workspaces
+    block.step(static)                                     # warm-up: plans of the calls, cuBLAS
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):

@@ -85,3 +85,32 @@ def test_step_from_a_captured_graph(cuda):
         assert block.lens.tolist() == [25, 12]
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D,H_q,H_kv,widths", [(128, 8, 2, (1, 2, 5, 16)), (64, 6, 3, (1, 32)), (256, 4, 1, (1, 16))])
+def test_steps_use_the_blocks_own_workspace(cuda, monkeypatch, D, H_q, H_kv, widths):
+    """Eager or captured, for steps of any width: no call makes a workspace (which a graph would fill again at each replay)."""
+    import torch
+
+    from kernelfoundry_b200 import kv_cache
+    from kernelfoundry_b200.q4_decode import Q4AttentionBlock
+
+    def none(*_):
+        raise AssertionError("the stream's workspace was asked for")
+
+    monkeypatch.setattr(kv_cache, "_workspace", none)
+    torch.manual_seed(3)
+    block = Q4AttentionBlock(2, 200, 256, H_q, H_kv, D, device=cuda)
+    block.prefill(torch.randn(2, 20, 256, device=cuda).half())
+    for w in widths:
+        x = torch.randn(2, w, 256, device=cuda).half()
+        block.step(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = block.step(x)
+        block.lens -= w                                  # the same step twice: eager, then replayed
+        want = block.step(x).clone()
+        block.lens -= w
+        graph.replay()
+        assert torch.equal(out, want)
