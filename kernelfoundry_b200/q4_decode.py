@@ -134,6 +134,8 @@ def main(argv=None):
     ap.add_argument("--prompt", type=int, default=2048)
     ap.add_argument("--steps", type=int, default=64)
     a = ap.parse_args(argv)
+    if a.batch < 1 or a.prompt < 2 or a.steps < 1:
+        ap.error("--batch and --steps must be at least 1, --prompt (two chunks) at least 2")
     torch.manual_seed(0)
     hidden, half = 4096, a.prompt // 2
     block = Q4AttentionBlock(a.batch, a.prompt + a.steps + 8, hidden)

@@ -54,3 +54,12 @@ def test_steps_after_a_capture_look_at_the_lengths():
     block.lens.copy_(torch.tensor([112, 0, 0]))
     with pytest.raises(ValueError, match="room for 112"):
         block.step(torch.zeros(3, 1, 64).half())
+
+
+@pytest.mark.parametrize("args", [("--steps", "0"), ("--prompt", "1"), ("--batch", "0")])
+def test_command_refuses_empty_runs(args, capsys):
+    from kernelfoundry_b200.q4_decode import main
+
+    with pytest.raises(SystemExit):
+        main(list(args))
+    assert "at least" in capsys.readouterr().err
