@@ -6,7 +6,8 @@ nvcc cross-compiles for B200 without a GPU.  The library links the static CUDA
 runtime and reaches the driver only through cudaGetDriverEntryPoint, so it
 loads (and its argument checks run) on machines without a GPU driver.  _kf_host.so is the
 host side of the small operators' Python calls (csrc/kf_host.cpp), built against the installed
-torch.
+torch.  It needs Python's and torch's headers; the library does not, and is built (and used from C)
+without them.
 """
 from __future__ import annotations
 
@@ -68,8 +69,7 @@ def build_host(force: bool = False) -> str:
     return HOST_PATH
 
 
-def build(verbose: bool = False, force: bool = False) -> str:
-    build_host(force)
+def build_library(verbose: bool = False, force: bool = False) -> str:
     if not force and not needs_rebuild():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -85,6 +85,16 @@ def build(verbose: bool = False, force: bool = False) -> str:
         raise RuntimeError(f"nvcc failed ({res.returncode}): {' '.join(cmd)}")
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
+
+
+def build(verbose: bool = False, force: bool = False) -> str:
+    """The library, then _kf_host.so; where that cannot be built, a warning (the calls that need it raise ImportError)."""
+    path = build_library(verbose, force)
+    try:
+        build_host(force)
+    except (OSError, RuntimeError) as e:
+        sys.stderr.write(f"warning: {path} is built, _kf_host.so is not, so the Python calls that need it will raise: {e}\n")
+    return path
 
 
 if __name__ == "__main__":
