@@ -14,7 +14,7 @@ import struct
 
 import torch
 
-from .build import HOST_PATH, LIB_PATH
+from .build import HOST_PATH, LIB_DIR, LIB_PATH
 
 KF_OK = 0
 KF_ERR_INVALID_ARG = 1
@@ -69,12 +69,13 @@ _host = None
 
 
 def host():
-    """Load _kf_host.so once (csrc/kf_host.cpp); raise if it has not been built."""
+    """Load _kf_host.so once (csrc/kf_host.cpp; beside the library, or the package's own); raise if it has not been built."""
     global _host
     if _host is None:
-        if not os.path.exists(HOST_PATH):
+        path = next((p for p in (HOST_PATH, os.path.join(LIB_DIR, os.path.basename(HOST_PATH))) if os.path.exists(p)), None)
+        if path is None:
             raise ImportError(f"{HOST_PATH} is missing: run `python -m kernelfoundry_b200.build`")
-        loader = importlib.machinery.ExtensionFileLoader("_kf_host", HOST_PATH)
+        loader = importlib.machinery.ExtensionFileLoader("_kf_host", path)
         _host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_kf_host", loader))
         loader.exec_module(_host)
     return _host

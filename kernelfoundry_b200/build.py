@@ -21,7 +21,7 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.environ.get("KF_LIB_PATH") or os.path.join(LIB_DIR, "libkf_attn.so")
-HOST_PATH = os.path.join(LIB_DIR, "_kf_host.so")
+HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(LIB_PATH)), "_kf_host.so")     # beside the library
 HOST_SOURCE = os.path.join(CSRC, "kf_host.cpp")
 SOURCES = ["kf_api.cu"]
 HEADERS = ["kf_ptx.cuh", "prefill_sm100.cuh", "decode_sm100.cuh", "pointwise_sm100.cuh", "peer_sm100.cuh",
@@ -54,7 +54,7 @@ def build_host(force: bool = False) -> str:
         return HOST_PATH
     import torch
 
-    os.makedirs(LIB_DIR, exist_ok=True)
+    os.makedirs(os.path.dirname(HOST_PATH), exist_ok=True)
     base, tmp = os.path.dirname(torch.__file__), HOST_PATH + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I" + sysconfig.get_paths()["include"],

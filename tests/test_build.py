@@ -2,8 +2,18 @@
 from __future__ import annotations
 
 import os
+import subprocess
+import sys
 
 import pytest
+
+from conftest import REPO
+
+
+def _python(code, **env):
+    res = subprocess.run([sys.executable, "-c", code], cwd=REPO, env={**os.environ, **env}, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr
+    return res.stdout.strip()
 
 
 @pytest.mark.parametrize("error", [RuntimeError("g++ failed (1): Python.h"), FileNotFoundError("g++")])
@@ -17,3 +27,16 @@ def test_library_is_built_without_pythons_headers(kf_lib, monkeypatch, capsys, e
     monkeypatch.setattr(build, "build_host", fail)
     assert build.build() == build.LIB_PATH and os.path.exists(build.LIB_PATH)
     assert str(error) in capsys.readouterr().err
+
+
+def test_a_library_elsewhere_has_its_module_beside_it(kf_lib, tmp_path):
+    """With KF_LIB_PATH nothing is built into the package's own lib/; a library without a module uses the package's."""
+    from kernelfoundry_b200 import build
+
+    lib = tmp_path / "libkf_attn.so"
+    lib.symlink_to(os.path.abspath(build.LIB_PATH))
+    where = "from kernelfoundry_b200 import build; print(build.HOST_PATH)"
+    assert os.path.dirname(_python(where, KF_LIB_PATH=str(lib))) == str(tmp_path)
+    assert os.path.dirname(_python(where, KF_LIB_PATH="")) == build.LIB_DIR
+    assert _python("from kernelfoundry_b200._lib import host; print(host().form())", KF_LIB_PATH=str(lib)) == "b''"
+    assert os.listdir(tmp_path) == ["libkf_attn.so"]
