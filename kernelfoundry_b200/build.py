@@ -1,10 +1,10 @@
-"""Build libkf_attn.so (sm_100a only) and _kf_host.so in-tree.
+"""Build libkf_attn.so (sm_100a only) and _kf_host-*.so in-tree.
 
     python -m kernelfoundry_b200.build [--verbose]
 
 nvcc cross-compiles for B200 without a GPU.  The library links the static CUDA
 runtime and reaches the driver only through cudaGetDriverEntryPoint, so it
-loads (and its argument checks run) on machines without a GPU driver.  _kf_host.so is the
+loads (and its argument checks run) on machines without a GPU driver.  _kf_host-*.so is the
 host side of the small operators' Python calls (csrc/kf_host.cpp), built against the installed
 torch.  It needs Python's and torch's headers; the library does not, and is built (and used from C)
 without them.
@@ -16,12 +16,16 @@ import subprocess
 import sys
 import sysconfig
 
+import torch
+
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.environ.get("KF_LIB_PATH") or os.path.join(LIB_DIR, "libkf_attn.so")
-HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(LIB_PATH)), "_kf_host.so")     # beside the library
+# Beside the library; named after the torch and the Python whose binary interfaces it is built against.
+HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(LIB_PATH)),
+                         f"_kf_host-torch{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
 HOST_SOURCE = os.path.join(CSRC, "kf_host.cpp")
 SOURCES = ["kf_api.cu"]
 HEADERS = ["kf_ptx.cuh", "prefill_sm100.cuh", "decode_sm100.cuh", "pointwise_sm100.cuh", "peer_sm100.cuh",
@@ -52,8 +56,6 @@ def needs_rebuild() -> bool:
 def build_host(force: bool = False) -> str:
     if not force and os.path.exists(HOST_PATH) and os.path.getmtime(HOST_PATH) >= os.path.getmtime(HOST_SOURCE):
         return HOST_PATH
-    import torch
-
     os.makedirs(os.path.dirname(HOST_PATH), exist_ok=True)
     base, tmp = os.path.dirname(torch.__file__), HOST_PATH + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",

@@ -40,3 +40,18 @@ def test_a_library_elsewhere_has_its_module_beside_it(kf_lib, tmp_path):
     assert os.path.dirname(_python(where, KF_LIB_PATH="")) == build.LIB_DIR
     assert _python("from kernelfoundry_b200._lib import host; print(host().form())", KF_LIB_PATH=str(lib)) == "b''"
     assert os.listdir(tmp_path) == ["libkf_attn.so"]
+
+
+def test_module_belongs_to_one_torch(kf_lib):
+    """Another torch or Python means another file: it is built anew there, and one built for another is never loaded."""
+    import sysconfig
+
+    import torch
+
+    from kernelfoundry_b200 import build
+
+    name = os.path.basename(build.HOST_PATH)
+    assert torch.__version__ in name and name.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+    code = ("import torch; torch.__version__ = '0.0.1'; from kernelfoundry_b200 import _lib, build\n"
+            "assert build.HOST_PATH != %r\ntry: _lib.host()\nexcept ImportError as e: print(e)" % build.HOST_PATH)
+    assert "0.0.1" in _python(code)
