@@ -54,7 +54,10 @@ def needs_rebuild() -> bool:
 
 
 def build_host(force: bool = False) -> str:
-    if not force and os.path.exists(HOST_PATH) and os.path.getmtime(HOST_PATH) >= os.path.getmtime(HOST_SOURCE):
+    built = os.path.exists(HOST_PATH)
+    if built and os.path.getmtime(HOST_PATH) < os.path.getmtime(HOST_SOURCE):
+        os.remove(HOST_PATH)                               # never loaded again, even if the build fails
+    elif built and not force:
         return HOST_PATH
     os.makedirs(os.path.dirname(HOST_PATH), exist_ok=True)
     base, tmp = os.path.dirname(torch.__file__), HOST_PATH + ".tmp"

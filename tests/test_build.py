@@ -55,3 +55,20 @@ def test_module_belongs_to_one_torch(kf_lib):
     code = ("import torch; torch.__version__ = '0.0.1'; from kernelfoundry_b200 import _lib, build\n"
             "assert build.HOST_PATH != %r\ntry: _lib.host()\nexcept ImportError as e: print(e)" % build.HOST_PATH)
     assert "0.0.1" in _python(code)
+
+
+def test_a_failed_build_leaves_no_outdated_module(monkeypatch, tmp_path):
+    """A module older than its source goes even if the new one cannot be built; an up-to-date one stays."""
+    from kernelfoundry_b200 import build
+
+    source, module = tmp_path / "kf_host.cpp", tmp_path / "_kf_host.so"
+    source.write_text("not C++")
+    module.write_text("")
+    monkeypatch.setattr(build, "HOST_SOURCE", str(source))
+    monkeypatch.setattr(build, "HOST_PATH", str(module))
+    os.utime(module, (os.path.getmtime(source) + 5,) * 2)
+    assert build.build_host() == str(module)
+    os.utime(module, (os.path.getmtime(source) - 5,) * 2)
+    with pytest.raises(RuntimeError, match="g"):
+        build.build_host()
+    assert not module.exists()
