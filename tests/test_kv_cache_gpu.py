@@ -650,3 +650,65 @@ def test_refused_workspaces(cuda):
     with pytest.raises(KFError):
         flash_attn_paged_q4(*args, workspace=good[:1024])
     assert torch.equal(flash_attn_paged_q4(*args, workspace=good), want)
+
+
+# ------------------------------------------------------------------ sizes at which a thread or a warp goes on to the next
+LARGE_IO = [
+    # B, S, H, D, block_size, dtype: rows for two passes of a write's block and four of a read's
+    (1, 5431, 7, 128, 16, "f16"),
+    (3, 1700, 8, 128, 64, "bf16"),
+    (2, 9503, 4, 64, 32, "bf16"),
+    (1, 2413, 8, 256, 128, "f16"),
+]
+
+
+@pytest.mark.parametrize("case", LARGE_IO, ids=lambda c: "B{}_S{}_H{}_D{}_bs{}_{}".format(*c))
+@pytest.mark.parametrize("layout", ["bhsd", "bshd"])
+def test_write_and_read_of_several_passes(cuda, case, layout):
+    B, S, H, D = case[:4]
+    assert B * S * 2 * H >= 4 * (4096 // D) * 4 * 148    # where both launchers begin to give a block all its passes
+    test_write_bytes_and_read_values(cuda, case, layout)
+
+
+def _alternating(cuda, rng, cache, table, B, H_q, S_q, D, lens, dt, out_dt, causal, check):
+    """B sequences on the pages of one: lengths and queries alternate between two, results against the oracle for all."""
+    q = po.round_to(rng.standard_normal((2, H_q, S_q, D)), dt)
+    O, _, _, A = qo.attention(q, cache, np.repeat(table, 2, 0), lens, causal)
+    pick = np.arange(B) % 2
+    got = _attn(cuda, q[pick], dt, cache, np.repeat(table, B, 0), np.array(lens)[pick], causal=causal, out_dtype=_tdt(out_dt))
+    check(got, O[pick], A[pick], out_dt, "")
+
+
+@pytest.mark.parametrize("D,H_q,S_q,B,dt,out_dt", [(128, 8, 1, 64, "f16", "f16"), (128, 5, 1, 64, "bf16", "bf16"), (64, 4, 1, 84, "f16", "f32"),
+                                                   (64, 2, 8, 64, "f16", "f16"), (128, 4, 4, 44, "f16", "f16"), (128, 4, 3, 44, "bf16", "bf16"),
+                                                   (256, 4, 2, 44, "f16", "f16"), (256, 1, 1, 44, "bf16", "bf16")])
+@pytest.mark.parametrize("bs", [16, 128])
+def test_warps_with_more_than_a_window_of_tiles(cuda, D, H_q, S_q, B, dt, out_dt, bs):
+    """Shares of 33 tiles and more for every warp: each ring stage is filled many times, the window of 32 tiles moves on,
+    and the maximum (by 58 bits) and the values' scales (by 2^20) grow again and again inside a share."""
+    rng = np.random.default_rng(D + 10 * H_q + S_q + bs)
+    n = 32000
+    warps = {(64, False): 16, (64, True): 12, (128, False): 12, (128, True): 8, (256, False): 8, (256, True): 8}[D, H_q * S_q > 8]
+    assert B * (n // 32) * (2 if D == 256 and H_q * S_q > 8 else 1) >= 33 * warps * 148
+    cache, table = _filled(rng, 1, 1, D, bs, [n])
+    _alternating(cuda, rng, cache, table, B, H_q, S_q, D, [n, n - 37], dt, out_dt, S_q > 1, _check)
+    u = np.sign(rng.standard_normal(D))
+    j = np.arange(n)
+    k = (40 / np.sqrt(D)) * (j % 1000 / 1000)[:, None] * u + 0.1 * rng.standard_normal((n, D))
+    v = rng.standard_normal((n, D)) * 2.0 ** np.floor(20 * (j % 700 / 700) - 15)[:, None]
+    slots = (table[0, j // bs] * bs + j % bs)[None].astype(np.int32)
+    cache = qo.write(cache, slots, k[None, None].astype(np.float32), v[None, None].astype(np.float32))
+    q = po.round_to(np.stack([np.broadcast_to(f * u, (H_q, S_q, D)) for f in (1.0, 0.5)]), dt)
+    O, _, _, A = qo.attention(q, cache, np.repeat(table, 2, 0), [n, n - 37], S_q > 1)
+    pick = np.arange(B) % 2
+    got = _attn(cuda, q[pick], dt, cache, np.repeat(table, B, 0), np.array([n, n - 37])[pick], causal=S_q > 1, out_dtype=_tdt(out_dt))
+    _check_rows(got, O[pick], A[pick], out_dt, "growing")
+
+
+@pytest.mark.parametrize("D,H_q,S_q", [(64, 8, 1), (128, 8, 1), (128, 4, 4), (256, 8, 1)])
+def test_full_batches_of_equal_lengths(cuda, D, H_q, S_q):
+    """64 sequences of 4096 keys with 8 cache heads: whole units and units cut between CTAs, several to a warp's share."""
+    rng = np.random.default_rng(D + S_q)
+    H, n = 8, 4096
+    cache, table = _filled(rng, 1, H, D, 16, [n])
+    _alternating(cuda, rng, cache, table, 64, H_q * H, S_q, D, [n, n], "f16", "f16", S_q > 1, _check)

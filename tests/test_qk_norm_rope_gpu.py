@@ -186,3 +186,34 @@ def test_refusals(cuda):
     narrow = torch.zeros(2, 4, 8, 132, device=cuda, dtype=torch.float16)[..., :128]
     with pytest.raises(KFError, match="invalid"):
         qk_norm_rope(narrow, None, None, None)
+
+
+LARGE = [
+    # groups of 8 tokens (4 where D = 512, 2), and blocks that go on to a second and a third group
+    (1, 2500, 3, 1, 128, 128, False, "f16"),
+    (1, 5003, 3, 2, 128, 64, False, "bf16"),
+    (2, 4999, 2, 1, 64, 64, True, "f16"),
+    (3, 1701, 1, 1, 256, 256, False, "f16"),
+    (1, 2417, 1, 1, 512, 512, False, "bf16"),
+    (700, 1, 4, 1, 128, 128, False, "f16"),
+    (1, 9999, 1, 1, 80, 16, False, "f16"),
+    (1, 2400, 41, 3, 96, 96, True, "bf16"),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: "B{}_S{}_Hq{}_Hkv{}_D{}_r{}_{}_{}".format(*c))
+def test_groups_of_tokens_and_blocks_with_several(cuda, case):
+    test_qk_norm_rope_matches_oracle(cuda, case)
+
+
+def test_groups_of_tokens_in_place_and_out_of_place_agree(cuda):
+    """5000 tokens (blocks take two groups): rows read for one group are not what another has written."""
+    import torch
+
+    from kernelfoundry_b200 import qk_norm_rope
+
+    torch.manual_seed(6)
+    q, k = (torch.randn(1, 5000, h, 128, device=cuda).half() for h in (5, 2))
+    a, b = qk_norm_rope(q, k, None, None, layout="bshd")
+    qk_norm_rope(q, k, None, None, layout="bshd", out=(q, k))
+    assert torch.equal(a, q) and torch.equal(b, k)
