@@ -45,8 +45,8 @@ extern "C" {
 
 /* Quantises k and v (both [B, H_kv, S, D] by element strides, head dimension contiguous)
  * into the cache: token (b, s) goes to slot slots[b * S + s].  A slot outside
- * [0, n_blocks * block_size) is skipped (padding: -1).  If one slot is named twice, either
- * token's K and V may end there.  strides: 6 values in host memory, the batch, head and token
+ * [0, n_blocks * block_size) is skipped (padding: -1).  If one slot is named twice, what ends there
+ * is undefined (it may be made of both tokens).  strides: 6 values in host memory, the batch, head and token
  * strides of k, then of v; multiples of 8, >= 0 (of a dimension of one element: any).
  * B * S == 0 is a no-op. */
 int kf_kv_write_q4(const void* k, const void* v, void* cache, const int* slots, int B, int S, int H_kv, int D,
@@ -60,7 +60,7 @@ int kf_kv_read_q4(const void* cache, const int* slots, void* k, void* v, int B, 
 
 /* Attention over the cache: O[b, h, i] = softmax_j(scale * q . k_j) v_j over the keys
  * j < seq_lens[b] of sequence b, whose logical block n is pool block
- * block_table[b * max_blocks + n].  Q and O [B, H_q, S_q, D] contiguous, query head h uses
+ * block_table[b * max_blocks + n].  Q and O [B, H_q, S_q, D] contiguous and without overlap, query head h uses
  * cache head h / (H_q / H_kv); H_q / H_kv * S_q at most 64 (longer chunks: kf_kv_read_q4 and
  * kf_attn_fwd_ex).  seq_lens is clamped to [0, max_blocks * block_size].
  * flags: KF_FLAG_CAUSAL: query i sees keys j <= seq_lens[b] - S_q + i; KF_FLAG_Q_BF16;
@@ -69,7 +69,8 @@ int kf_kv_read_q4(const void* cache, const int* slots, void* k, void* v, int B, 
  * Table entries past a sequence's last block are not read; an entry outside
  * [0, n_blocks) reads zeros.  Probabilities times the values' scales enter the second
  * product as fp16 for a bf16 O (2^-11 a key, relative) and as two fp16 for fp16 and fp32 (2^-22),
- * in both cases to no finer than 2^-23 of the row's largest; everything else is exact or fp32.  max_blocks * block_size < 2^31 - 64.
+ * in both cases to no finer than 2^-23 of the row's largest; everything else is exact or fp32
+ * (for queries below 2^120: beyond, scores may overflow that would not have to).  max_blocks * block_size < 2^31 - 64.
  * workspace: required, kf_attn_paged_q4_workspace_bytes(), handled as kf_attn_fwd's
  * (zero-filled once, left ready by every call, not shared by overlapping calls);
  * KF_ERR_WORKSPACE if it is too small. */

@@ -6,8 +6,10 @@
 // What bounds it: a key and value of one head are D + 8 bytes, read once; at 6.5 TB/s an SM
 // receives 46 codes per clock, so the codes have to become MMA operands in about two
 // instructions per eight.  mma.m16n8k16 with the KEYS as its 16 rows and the queries as its 8
-// columns (S^T = K Q^T, O^T = V^T P^T) wastes nothing for up to 8 query rows a cache head; the
-// 128-row tcgen05 tiles would be 1/16 filled and want their operands expanded in memory.
+// columns (S^T = K Q^T, O^T = V^T P^T) wastes nothing for up to 8 query rows a cache head; a
+// 128-row tcgen05 tile would be 1/16 filled by 8 rows (half by the 64 that are accepted) and wants
+// its operands expanded in memory.  Beyond 8 NT rows every group of them copies and unpacks the
+// cache for itself (B=32, 4096 keys of 128: 8 rows 40.1 us, 16 60.1, 32 109, 64 203).
 //
 // Codes to operands.  A 4-bit integer in bits 2..5 of an fp16 is the subnormal n * 2^-22, in bits
 // 6..9 it is n * 2^-18, and the tensor core multiplies subnormals exactly.  For K two shifts and
@@ -19,8 +21,9 @@
 // For V two keys' words are interleaved by halves (prmt), masked in place (bits 0..3 and 4..7), and
 // one half2 FMA makes (n - z) * 2^-9 of each pair, exact and normal: sums of p t (n - z) keep the
 // value's own size, where sum(p t n) - sum(p t z) would cancel.
-// Queries are scaled by a power of two per row to a maximum in [2^13, 2^14), which holds fp16
-// rows exactly, and bf16 ones but for elements below 2^-28 of the row's largest.
+// Queries are scaled by a power of two per row to a maximum in [2^13, 2^14), every other operand
+// by 1/16 of it.  fp16's last bit is then 2^-37 of the row's largest element, or 2^-33 in those:
+// what is lost of an element is at most half of that.
 // p t enters the second product as fp16, times a power of two (norm) of its query row: the one that
 // keeps the largest t seen below 2^7, or a larger one if the row's largest p t would then be below
 // 2^-2 (a value far beyond the others with next to no probability, or hidden from the row, must not
@@ -43,10 +46,11 @@
 // timing).
 //
 // Measured, 32 query and 8 cache heads of 128 (bytes of codes and words over time; 6.55 TB/s is a copy):
-// B=64, KV=4096 66.5 us (4.3 TB/s), B=16 25.2 (2.8), B=1, KV=131072 38.4 (3.7), B=1, KV=512 8.0.  The copies
-// alone take 46 us at B=64 and 24.6 at KV=131072; the rest is instructions (293 for 16 keys, at 2.2
-// to 2.4 a clock, the ALU pipe busiest) and, for few sequences, the chain of loads before the first
-// tile (about 6000 clocks) and the merges.
+// B=64, KV=4096 69.9 us (4.1 TB/s; bf16 65.9), B=16 25.7 (2.8), B=1, KV=131072, bf16 38.2 (3.7), B=1, KV=512
+// 8.3.  The copies alone take 46 us at B=64 and 24.6 at KV=131072.  The rest is latency inside a warp: 296
+// instructions for 16 keys form one chain (scores, exponentials, transposition, values' products), and 3 warps
+// a scheduler issue 1.9 of 4 a clock at B=16 with no pipe more than 42 % busy (ALU; tensor 27 %); for few
+// sequences it is the chain of loads before the first tile (about 6000 clocks) and the merges.
 #pragma once
 
 #include "cache_sm100.cuh"
@@ -75,8 +79,9 @@ struct Q4AttnParams {
 template <int D_, int NT_>
 struct Q4AttnCfg {
     static constexpr int D = D_, NT = NT_;
-    // As many warps as the registers allow without spills (D = 64 with 12 warps: 51.2 us instead of 45.8 at
-    // B=32, KV=8192; D = 128 with 16: 128 registers, which spill).  Two stages hide the copies; a third
+    // As many warps as the registers allow without spills in the loop (D = 64 with 12 warps: 51.2 us instead of
+    // 45.8 at B=32, KV=8192; D = 128 with 16: 128 registers, which spill; D = 64 with 16 rows and two operands
+    // of p spills 4 bytes).  Two stages hide the copies; a third
     // costs 0 to 2 % at 12 warps of 8 rows and gains 2 % at 8 warps of 16.
     static constexpr int W = D == 256 ? 8 : NT == 1 ? (D == 64 ? 16 : 12) : (D == 64 ? 12 : 8);   // warps
     static constexpr int STAGES = NT == 2 || D == 64 ? 3 : 2;
@@ -543,11 +548,17 @@ __device__ __forceinline__ void q4_emit(const Q4AttnParams& p, Q4Warp<D, NT>& s,
     }
 }
 
-// What the merge of a unit across CTAs costs, in tiles of one CTA.  (With 0, an even split whenever it is
-// shorter: B=1, KV=512 9.0 us instead of 8.0, B=16, KV=4096 25.7 instead of 25.2.)
+// What the merge of a unit across CTAs costs, in tiles of one CTA.  Fitted at D = 128 and good for the others:
+// B=16, 8 cache heads, with 0 (an even split whenever it is shorter) / 32 / 64, in us:
+//   rows x D    KV=2048              KV=4096              KV=8192
+//   4 x 64      15.0 / 13.5 / 13.3   19.5 / 18.5 / 18.4   28.7 / 28.4 / 28.7
+//   4 x 128     17.9 / 16.8 / 16.9   25.6 / 25.2 / 25.1   39.8 / 39.8 / 41.9
+//   4 x 256     26.9 / 25.4 / 25.2   39.9 / 40.5 / 40.4   65.4 / 65.6 / 71.0
+//   16 x 64     19.1 / 16.4 / 16.4   26.4 / 24.1 / 24.1   40.3 / 40.0 / 40.2
+//   16 x 128    24.9 / 23.1 / 23.1   36.3 / 36.6 / 36.6   59.2 / 59.0 / 63.6
 constexpr unsigned kQ4MergeTiles = 32;
 // What a unit costs a warp besides its tiles (queries in, results out), in tiles.  (With 0: 48 sequences
-// of 1 to 8192 keys 24.6 us instead of 18.2.)
+// of 1 to 8192 keys 24.6 us instead of 18.3.)
 constexpr int kQ4UnitTiles = 2;
 
 __device__ __forceinline__ float q4_weight(float m, float M) { return m == -INFINITY ? 0.f : ex2_approx(m - M); }
@@ -676,8 +687,9 @@ __global__ void __launch_bounds__(Q4AttnCfg<D, NT>::THREADS, 1) q4_attn_kernel(c
         if (lane >= o) incl += v;
     }
     const unsigned T = __shfl_sync(0xffffffffu, incl, 31) * HR;          // < 2^31, the host sees to it
-    // CTAs that take part: every warp of theirs gets at least a slot.  CTA c has the slots from
-    // c * quot + min(c, rem), its warps even shares of them.
+    // CTAs that take part: about a slot for every warp of theirs at least.  CTA c has the slots from
+    // c * quot + min(c, rem), its warps even shares of them; where there are fewer slots than warps, the
+    // last warps are the ones without (the merge below relies on a unit's warps being neighbours).
     const unsigned want = (T + W - 1) / W;
     unsigned act = want < gridDim.x ? want : gridDim.x, quot = T / act, rem = T - quot * act;
     // Sequences of one length: whole units to each CTA, if that takes no longer than an even

@@ -89,7 +89,7 @@ def kv_write_q4(k, v, cache, slots, *, layout: str = "bhsd") -> None:
     k, v: fp16 or bf16, ``[B, H_kv, S, D]`` ("bhsd") or ``[B, S, H_kv, D]`` ("bshd"), any
     strides (multiples of 8) with a contiguous head dimension.  slots: int32 ``[B, S]``; slot
     t is row ``t % block_size`` of block ``t // block_size``; one outside the cache (-1) is
-    skipped.  Each head row is quantised by itself (scale and zero point per row)."""
+    skipped, one named twice holds anything.  Each head row is quantised by itself (scale and zero point per row)."""
     h = host()
     key = (layout, h.form(k, v, cache, slots))
     index, plan = _write_plans.get(key) or _write_plans.put(key, _plan_io(lib().kf_kv_write_q4, cache, slots, k, v, layout))
@@ -116,7 +116,7 @@ def _plan_io(fn, cache, slots, k, v, layout):
 def kv_read_q4(cache, slots, *, dtype=torch.float16, layout: str = "bhsd", out=None):
     """``(k, v)`` of the tokens in ``slots`` (int32 ``[B, S]``) as fp16 or bf16 tensors.
 
-    ``[B, H_kv, S, D]`` ("bhsd", what :func:`flash_attn_fwd` takes) or ``[B, S, H_kv, D]``
+    ``[B, H_kv, S, D]`` ("bhsd", in fp16 what :func:`flash_attn_fwd` takes) or ``[B, S, H_kv, D]``
     ("bshd").  A slot outside the cache reads zeros.  ``out``: (k, v) to write into."""
     h = host()
     if out is None:
