@@ -69,7 +69,7 @@ _host = None
 
 
 def host():
-    """Load _kf_host.so once (csrc/kf_host.cpp; beside the library, or the package's own); raise if it has not been built."""
+    """Load _kf_host-*.so once (csrc/kf_host.cpp; beside the library, or the package's own); raise if it has not been built."""
     global _host
     if _host is None:
         path = next((p for p in (HOST_PATH, os.path.join(LIB_DIR, os.path.basename(HOST_PATH))) if os.path.exists(p)), None)

@@ -93,12 +93,12 @@ def build_library(verbose: bool = False, force: bool = False) -> str:
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
-    """The library, then _kf_host.so; where that cannot be built, a warning (the calls that need it raise ImportError)."""
+    """The library, then _kf_host-*.so; where that cannot be built, a warning (the calls that need it raise ImportError)."""
     path = build_library(verbose, force)
     try:
         build_host(force)
     except (OSError, RuntimeError) as e:
-        sys.stderr.write(f"warning: {path} is built, _kf_host.so is not, so the Python calls that need it will raise: {e}\n")
+        sys.stderr.write(f"warning: {path} is built, _kf_host-*.so is not, so the Python calls that need it will raise: {e}\n")
     return path
 
 
