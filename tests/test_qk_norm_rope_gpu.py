@@ -189,7 +189,7 @@ def test_refusals(cuda):
 
 
 LARGE = [
-    # groups of 8 tokens (4 where D = 512, 2), and blocks that go on to a second and a third group
+    # groups of 8 tokens (4 at D = 512, 2 for 700 sequences), and blocks that go on to a second and a third group
     (1, 2500, 3, 1, 128, 128, False, "f16"),
     (1, 5003, 3, 2, 128, 64, False, "bf16"),
     (2, 4999, 2, 1, 64, 64, True, "f16"),
